@@ -44,7 +44,8 @@ typedef enum sofie_b200_status {
   SOFIE_B200_ERR_CUDA = -2,        /* a CUDA runtime or driver call failed               */
   SOFIE_B200_ERR_DEVICE_WAIT = -3, /* a bounded wait inside a kernel gave up             */
   SOFIE_B200_ERR_NO_DEVICE = -4,   /* no sm_100 device / driver entry point unavailable  */
-  SOFIE_B200_ERR_TOO_LARGE = -5    /* size beyond a documented static limit              */
+  SOFIE_B200_ERR_TOO_LARGE = -5,   /* size beyond a documented static limit              */
+  SOFIE_B200_ERR_DEVICE_INDEX = -6 /* an index in device memory (a page, a length, an offset) was out of range */
 } sofie_b200_status;
 
 /* Element types.  The reference's ETensorType (core/inc/SOFIE/utils/SOFIE_common.hxx:29-32)
@@ -226,7 +227,9 @@ int sofie_b200_ctx_destroy(sofie_b200_ctx *ctx);
 
 /* Waits for the stream (the alpaka::wait(queue) at the end of Session::infer,
  * RModel_ALPAKA.cxx:857-909) and returns SOFIE_B200_ERR_DEVICE_WAIT if a kernel reported a
- * bounded wait that ran out since the last call. */
+ * bounded wait that ran out since the last call, or SOFIE_B200_ERR_DEVICE_INDEX if one met a page, length or
+ * offset in device memory that is out of range (the generation operators check what they read from
+ * block tables and length arrays, leave out the access, and carry on). */
 int sofie_b200_ctx_sync(sofie_b200_ctx *ctx);
 
 /* Number of kernels this ctx has launched so far (for launch accounting in benchmarks). */
@@ -407,6 +410,100 @@ const char *sofie_b200_sdpa_plan_kernel(const sofie_b200_sdpa_plan *plan);
 int64_t sofie_b200_sdpa_workspace_bytes(const sofie_b200_sdpa_plan *plan);
 int sofie_b200_sdpa_enqueue(sofie_b200_sdpa_plan *plan, const void *q, const void *k, const void *v, const void *mask, void *y,
                             void *workspace);
+
+/* ---- generation: a paged key-value cache and the attention over it ------------------------------------------------
+ *
+ * (The reference has no counterpart: its ROperator_SDPA, core/inc/SOFIE/operators/ROperator_SDPA.hxx:38-330, knows one dense
+ * batch of equal lengths, as many key heads as query heads and no causal order.)  Three operators share one description of
+ * a batch of sequences, all of it in device memory, so that a step captured into a CUDA graph is replayed for other lengths:
+ *   cu_seqlens   int32 [batch + 1]: the rows [cu_seqlens[b], cu_seqlens[b+1]) of a packed [tokens, heads, head_dim] tensor belong
+ *                to sequence b; rows from cu_seqlens[batch] on belong to nobody and are neither read into a result nor written
+ *   seq_lens     int32 [batch]: tokens of sequence b in the cache, the ones being appended included
+ *   block_table  int32 [batch, table_width]: token p of sequence b lives in page block_table[b][p / page_size], slot p % page_size
+ * Grouped heads: query head h reads key head h / (heads / kv_heads).  Types F32 and BF16, one for all tensors of a call; scores,
+ * row maxima, row sums and results are held in fp32 and rounded once.
+ * Indices in device memory cannot be refused by the host.  The kernels check them: a token whose page, position or row is out of
+ * range is left out (not written, not attended to), every other one is processed, and the next sofie_b200_ctx_sync returns
+ * SOFIE_B200_ERR_DEVICE_INDEX.
+ */
+typedef struct sofie_b200_paged_kv {
+  void *k, *v;                   /* element (page, slot, head, d) at page * page_stride + slot * token_stride + head * head_stride + d */
+  const int32_t *block_table;    /* [batch, table_width], rows table_pitch apart */
+  const int32_t *seq_lens;       /* [batch] */
+  int64_t batch;
+  int64_t num_pages;
+  int64_t table_width, table_pitch;               /* table_pitch 0 = table_width */
+  int64_t page_stride, token_stride, head_stride; /* elements; all 0 = dense [num_pages, page_size, kv_heads, head_dim] */
+  int32_t page_size;             /* any size from 1 */
+} sofie_b200_paged_kv;
+
+/* Appends the new tokens' keys and values to the cache; on the way the first rotary_dim dimensions of every key head (and query
+ * head) are rotated by the token's position p = seq_lens[b] - (new tokens of b) + i, as ONNX RotaryEmbedding defines it:
+ *   interleaved = 0   (x[j], x[j + r/2]) -> (x[j] cos[p][j] - x[j + r/2] sin[p][j],  x[j + r/2] cos[p][j] + x[j] sin[p][j])
+ *   interleaved = 1   the same for the neighbours (x[2j], x[2j + 1])
+ * in fp32, rounded once; r = rotary_dim, 0 = no rotation (cos and sin NULL). */
+typedef struct sofie_b200_kv_append_desc {
+  int64_t tokens;                /* rows of q, k, v, q_out, k_out; cu_seqlens[batch] may be smaller */
+  int32_t heads;                 /* query heads; 0 = no q */
+  int32_t kv_heads, head_dim;
+  int32_t rotary_dim;            /* even, <= head_dim */
+  int32_t interleaved;
+  int32_t dtype;                 /* F32 or BF16 */
+  int64_t max_position;          /* rows of cos and sin */
+  int64_t ldq, ldk, ldv, ldqo, ldko;   /* token pitches in elements, 0 = dense */
+} sofie_b200_kv_append_desc;
+/* q [tokens, heads, head_dim] -> q_out, k and v [tokens, kv_heads, head_dim] -> the cache, and the rotated keys -> k_out too when
+ * it is not NULL (what sofie_b200_prompt_attention_enqueue reads).  cos, sin: F32 [max_position, rotary_dim / 2].  q_out may be q and
+ * k_out may be k (the same pointer and pitch); otherwise outputs overlap nothing.  cu_seqlens NULL: one token per sequence
+ * (tokens == batch), where seq_lens[b] = 0 marks a padding row that is skipped.  No two tokens of a call share a slot of the cache. */
+int sofie_b200_kv_append_enqueue(sofie_b200_ctx *ctx, const sofie_b200_kv_append_desc *desc, const sofie_b200_paged_kv *kv,
+                                 const int32_t *cu_seqlens, const void *q, const void *k, const void *v, const float *cos,
+                                 const float *sin, void *q_out, void *k_out);
+
+/* Attention over packed prompts: y[i,h] = sum_j softmax_j(scale q[i,h] . k[j, h / g]) v[j, h / g] over the keys j of query i's own
+ * sequence -- all lk of them, or with causal = 1 those with j <= i + lk - lq (the last query sees the last key; lk > lq: a prompt
+ * continued after lk - lq keys).  A query that sees no key gets zeros.  Keys and values that a query does not see have no
+ * influence on it, whatever they hold (NaN and infinities included).
+ * head_dim: a multiple of 8 up to 256; heads / kv_heads up to 64; token pitches multiples of 8 elements; tensors 16-byte aligned. */
+typedef struct sofie_b200_prompt_attention_desc {
+  int32_t heads, kv_heads, head_dim;
+  int32_t dtype;                 /* F32 or BF16 */
+  int32_t causal;
+  float scale;                   /* > 0, or 0 = 1 / sqrt(head_dim) */
+  int64_t ldq, ldk, ldv, ldy;    /* token pitches in elements, 0 = dense */
+} sofie_b200_prompt_attention_desc;
+typedef struct sofie_b200_prompt_attention_plan sofie_b200_prompt_attention_plan;
+int sofie_b200_prompt_attention_plan_create(sofie_b200_ctx *ctx, const sofie_b200_prompt_attention_desc *desc,
+                                            sofie_b200_prompt_attention_plan **out);
+int sofie_b200_prompt_attention_plan_destroy(sofie_b200_prompt_attention_plan *plan);
+const char *sofie_b200_prompt_attention_plan_kernel(const sofie_b200_prompt_attention_plan *plan);
+/* q, y: [q_tokens, heads, head_dim]; k, v: [k_tokens, kv_heads, head_dim].  cu_seqlens_k NULL = cu_seqlens_q. */
+int sofie_b200_prompt_attention_enqueue(sofie_b200_prompt_attention_plan *plan, const void *q, const void *k, const void *v, void *y,
+                                        const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int64_t batch, int64_t q_tokens,
+                                        int64_t k_tokens);
+
+/* Attention of one new token per sequence over the paged cache: y[b,h] = the sum above over the seq_lens[b] tokens of sequence b in
+ * the cache.  seq_lens[b] = 0 (a padding row) gives zeros.  The cache's length is split over the GPU whatever the batch is, and the
+ * parts are joined in a fixed order (the same inputs give the same bits).
+ * head_dim: a multiple of 8 up to 256; heads / kv_heads up to 64; strides and pitches multiples of 8 elements; tensors 16-byte aligned. */
+typedef struct sofie_b200_paged_attention_desc {
+  int32_t heads, kv_heads, head_dim;
+  int32_t dtype;                 /* F32 or BF16 */
+  float scale;                   /* > 0, or 0 = 1 / sqrt(head_dim) */
+  int64_t ldq, ldy;              /* row pitches in elements, 0 = dense */
+} sofie_b200_paged_attention_desc;
+typedef struct sofie_b200_paged_attention_plan sofie_b200_paged_attention_plan;
+int sofie_b200_paged_attention_plan_create(sofie_b200_ctx *ctx, const sofie_b200_paged_attention_desc *desc,
+                                           sofie_b200_paged_attention_plan **out);
+int sofie_b200_paged_attention_plan_destroy(sofie_b200_paged_attention_plan *plan);
+const char *sofie_b200_paged_attention_plan_kernel(const sofie_b200_paged_attention_plan *plan);
+/* Bytes of 256-byte aligned caller scratch for the parts of split sequences; depends on the plan alone, not on the batch or its
+ * lengths.  Its contents need no preparation and mean nothing between calls.  Calls that may run at the same time (two streams,
+ * two captured graphs replayed side by side) need a workspace each. */
+int64_t sofie_b200_paged_attention_workspace_bytes(const sofie_b200_paged_attention_plan *plan);
+/* q, y: [batch, heads, head_dim] (batch = kv->batch). */
+int sofie_b200_paged_attention_enqueue(sofie_b200_paged_attention_plan *plan, const void *q, const sofie_b200_paged_kv *kv, void *y,
+                                       void *workspace);
 
 /* ---- memory-bound operators the fusion pass leaves ----------------------------------- */
 

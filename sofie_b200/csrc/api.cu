@@ -110,6 +110,7 @@ const char *sofie_b200_status_string(int status) {
     case SOFIE_B200_ERR_DEVICE_WAIT: return "a bounded wait inside a kernel gave up";
     case SOFIE_B200_ERR_NO_DEVICE: return "no usable sm_100 device";
     case SOFIE_B200_ERR_TOO_LARGE: return "size beyond a static limit";
+    case SOFIE_B200_ERR_DEVICE_INDEX: return "an index in device memory was out of range";
   }
   return "unknown status";
 }
@@ -174,6 +175,8 @@ int sofie_b200_ctx_sync(sofie_b200_ctx *ctx) {
   if (s != 0) {
     cudaMemsetAsync(ctx->d_status, 0, sizeof(int), ctx->stream);
     cudaStreamSynchronize(ctx->stream);
+    if (s == DEV_BAD_INDEX)
+      return fail(SOFIE_B200_ERR_DEVICE_INDEX, "device status %d: a page, position or offset in device memory was out of range and was left out", s);
     return fail(SOFIE_B200_ERR_DEVICE_WAIT, "device status %d: %s", s, (s > 0 && s < 5) ? kDeviceWait[s] : "unknown");
   }
   return 0;

@@ -31,6 +31,7 @@ enum DeviceStatus : int {
   DEV_WAIT_SMEM_FULL = 2,   // MMA issuer waited for a filled stage
   DEV_WAIT_TMEM_EMPTY = 3,  // MMA issuer waited for a drained accumulator
   DEV_WAIT_TMEM_FULL = 4,   // epilogue waited for a finished accumulator
+  DEV_BAD_INDEX = 5,        // a page, length or offset read from device memory was out of range; the access was left out
 };
 
 inline int dtype_size(int dt) {

@@ -1,0 +1,68 @@
+// Index arithmetic of the generation operators (append to a paged cache, attention over packed prompts, attention over the
+// cache).  Plain integer functions, for the kernels and for a host compiler alike: tests/test_generate.py builds this
+// file with g++ and runs every function over hostile tables and lengths, because an index that leaves its buffer must be
+// found there and not on a GPU.
+#pragma once
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#define SB_HD __host__ __device__ __forceinline__
+#else
+#define SB_HD inline
+#endif
+
+namespace sb200 {
+
+// A paged cache and its sequences (sofie_b200_paged_kv with the defaults filled in).
+struct PagedView {
+  const int32_t *table;      // [batch, table_width], rows table_pitch apart
+  const int32_t *lens;       // [batch]
+  long long table_pitch;
+  long long page_stride, token_stride, head_stride;   // elements
+  int batch, num_pages, table_width, page_size;
+};
+
+// Element offset of (position pos of sequence b, head 0) in the cache, or -1 when the position has no page or the page does not
+// exist.  64-bit throughout: a cache of 2^31 elements is 4 GB of bf16.
+SB_HD long long paged_row(const PagedView &c, int b, int pos) {
+  if (pos < 0) return -1;
+  const int page_index = pos / c.page_size;
+  if (page_index >= c.table_width) return -1;
+  const int page = c.table[(long long)b * c.table_pitch + page_index];
+  if (page < 0 || page >= c.num_pages) return -1;
+  return (long long)page * c.page_stride + (long long)(pos - page_index * c.page_size) * c.token_stride;
+}
+
+// Tokens of sequence b that the cache can hold and the length array claims; `bad` is set when the array claims others.
+SB_HD int paged_len(const PagedView &c, int b, bool *bad) {
+  const int n = c.lens[b];
+  const long long room = (long long)c.table_width * c.page_size;
+  if (n < 0) { *bad = true; return 0; }
+  if (n > room) { *bad = true; return (int)room; }
+  return n;
+}
+
+// Rows [*begin, *end) of sequence b in a packed tensor of `rows` rows, empty and *bad when the offsets are not 0 <= begin <= end <= rows.
+SB_HD void packed_range(const int32_t *cu, int b, long long rows, int *begin, int *end, bool *bad) {
+  const int x = cu[b], y = cu[b + 1];
+  if (x < 0 || y < x || y > rows) {
+    *begin = *end = 0;
+    *bad = true;
+    return;
+  }
+  *begin = x;
+  *end = y;
+}
+
+// The sequence that row t belongs to (cu[b] <= t < cu[b + 1]), or -1.  Any contents of cu end the search inside [0, batch).
+SB_HD int packed_find(const int32_t *cu, int batch, int t) {
+  int lo = 0, hi = batch;   // invariant for an ordered cu: cu[lo] <= t or no sequence holds t
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (cu[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return batch > 0 && cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
+}
+
+}  // namespace sb200

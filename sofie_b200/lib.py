@@ -16,7 +16,7 @@ LIB_PATH = PKG / "libsofie_b200.so"
 F32, BF16, I8, F8E4M3, I32, U8 = range(6)
 ACT_NONE, ACT_RELU, ACT_GELU_ERF, ACT_GELU_TANH, ACT_LEAKY_RELU, ACT_SIGMOID = range(6)
 BIAS_NONE, BIAS_COL_F32, BIAS_ROW_F32, BIAS_SCALAR_F32, BIAS_COL_I32, BIAS_FULL_F32, BIAS_ROW_I32 = range(7)
-OK, ERR_INVALID, ERR_CUDA, ERR_DEVICE_WAIT, ERR_NO_DEVICE, ERR_TOO_LARGE = 0, -1, -2, -3, -4, -5
+OK, ERR_INVALID, ERR_CUDA, ERR_DEVICE_WAIT, ERR_NO_DEVICE, ERR_TOO_LARGE, ERR_DEVICE_INDEX = 0, -1, -2, -3, -4, -5, -6
 ABI_VERSION = 2
 GEMM_B_CONSTANT = 1
 GEMM_WIDE_STORES = 2
@@ -83,6 +83,44 @@ class SdpaDesc(C.Structure):
     ]
 
 
+class PagedKv(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("block_table", C.c_void_p), ("seq_lens", C.c_void_p),
+        ("batch", C.c_int64),
+        ("num_pages", C.c_int64),
+        ("table_width", C.c_int64), ("table_pitch", C.c_int64),
+        ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64),
+        ("page_size", C.c_int32),
+    ]
+
+
+class KvAppendDesc(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_int64),
+        ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("rotary_dim", C.c_int32), ("interleaved", C.c_int32), ("dtype", C.c_int32),
+        ("max_position", C.c_int64),
+        ("ldq", C.c_int64), ("ldk", C.c_int64), ("ldv", C.c_int64), ("ldqo", C.c_int64), ("ldko", C.c_int64),
+    ]
+
+
+class PromptAttentionDesc(C.Structure):
+    _fields_ = [
+        ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("dtype", C.c_int32), ("causal", C.c_int32), ("scale", C.c_float),
+        ("ldq", C.c_int64), ("ldk", C.c_int64), ("ldv", C.c_int64), ("ldy", C.c_int64),
+    ]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = [
+        ("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("dtype", C.c_int32), ("scale", C.c_float),
+        ("ldq", C.c_int64), ("ldy", C.c_int64),
+    ]
+
+
 class TensorLife(C.Structure):
     _fields_ = [("begin", C.c_int64), ("end", C.c_int64), ("size", C.c_int64)]
 
@@ -124,6 +162,16 @@ PROTOTYPES = {
     "sofie_b200_sdpa_plan_kernel": (C.c_char_p, [_P]),
     "sofie_b200_sdpa_workspace_bytes": (_I64, [_P]),
     "sofie_b200_sdpa_enqueue": (C.c_int, [_P, _P, _P, _P, _P, _P, _P]),
+    "sofie_b200_kv_append_enqueue": (C.c_int, [_P, C.POINTER(KvAppendDesc), C.POINTER(PagedKv), _P, _P, _P, _P, _P, _P, _P, _P]),
+    "sofie_b200_prompt_attention_plan_create": (C.c_int, [_P, C.POINTER(PromptAttentionDesc), C.POINTER(_P)]),
+    "sofie_b200_prompt_attention_plan_destroy": (C.c_int, [_P]),
+    "sofie_b200_prompt_attention_plan_kernel": (C.c_char_p, [_P]),
+    "sofie_b200_prompt_attention_enqueue": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64]),
+    "sofie_b200_paged_attention_plan_create": (C.c_int, [_P, C.POINTER(PagedAttentionDesc), C.POINTER(_P)]),
+    "sofie_b200_paged_attention_plan_destroy": (C.c_int, [_P]),
+    "sofie_b200_paged_attention_plan_kernel": (C.c_char_p, [_P]),
+    "sofie_b200_paged_attention_workspace_bytes": (_I64, [_P]),
+    "sofie_b200_paged_attention_enqueue": (C.c_int, [_P, _P, C.POINTER(PagedKv), _P, _P]),
     "sofie_b200_layernorm_enqueue": (C.c_int, [_P, _P, _P, _I32, _I32, _I64, _I64, _P, _P, _F, _P, _P]),
     "sofie_b200_softmax_enqueue": (C.c_int, [_P, _P, _P, _I32, _I32, _I64, _I64, _I32]),
     "sofie_b200_softmax_axis_enqueue": (C.c_int, [_P, _P, _P, _I32, _I64, _I64, _I64, _I32]),

@@ -183,6 +183,41 @@ class Context:
         L.check(self._lib.sofie_b200_attention_enqueue(self._h, _ptr(qkv), _ptr(out), dtype_code(qkv.dtype), batch, seq, heads, head_dim,
                                                        float(scale)), "attention_enqueue")
 
+    def kv_append(self, k, v, kv, cu_seqlens=None, cos=None, sin=None, interleaved=False, q=None, q_out=None, k_out=None):
+        """Appends keys and values of new tokens to a paged cache (`kv`, a PagedKV), rotating keys and queries by their positions
+        on the way.  k, v: [tokens, kv_heads, head_dim]; q, q_out: [tokens, heads, head_dim]; k_out: the rotated keys once more,
+        packed, for PromptAttentionPlan.  cos, sin: fp32 [positions, rotary_dim / 2], absent = no rotation.  cu_seqlens: int32
+        [batch + 1], the packed rows of each sequence; absent = one token per sequence.  Token rows may be column blocks of a
+        wider tensor.  q_out may be q, k_out may be k."""
+        tokens, kv_heads, dim, ldk = _rows("k", k)
+        if (kv_heads, dim) != (kv.kv_heads, kv.head_dim) or k.dtype != kv.dtype:
+            raise ValueError(f"kv_append: keys of {kv_heads} heads of {dim} {k.dtype}, cache of {kv.kv_heads} of {kv.head_dim} {kv.dtype}")
+        ldv = _same_rows("v", v, k)
+        ldko = _same_rows("k_out", k_out, k) if k_out is not None else 0
+        heads = ldq = ldqo = 0
+        if q is not None:
+            if q_out is None:
+                raise ValueError("kv_append: q needs q_out")
+            n, heads, qdim, ldq = _rows("q", q)
+            if n != tokens or qdim != dim or q.dtype != k.dtype:
+                raise ValueError("kv_append: q and k differ in tokens, head size or type")
+            ldqo = _same_rows("q_out", q_out, q)
+        elif q_out is not None:
+            raise ValueError("kv_append: q_out needs q")
+        rotary = positions = 0
+        if cos is not None or sin is not None:
+            if cos is None or sin is None or cos.shape != sin.shape or cos.dim() != 2 or not (cos.is_contiguous() and sin.is_contiguous()):
+                raise ValueError("kv_append: cos and sin are two contiguous tensors of one shape [positions, rotary_dim / 2]")
+            if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+                raise TypeError("kv_append: cos and sin are fp32")
+            positions, rotary = cos.shape[0], 2 * cos.shape[1]
+        if cu_seqlens is not None:
+            _offsets("cu_seqlens", cu_seqlens, kv.batch)
+        d = L.KvAppendDesc(tokens, heads, kv_heads, dim, rotary, int(interleaved), dtype_code(k.dtype), positions, ldq, ldk, ldv, ldqo, ldko)
+        L.check(self._lib.sofie_b200_kv_append_enqueue(
+            self._h, C.byref(d), kv._ref, _ptr(cu_seqlens), _ptr(q), _ptr(k), _ptr(v), _ptr(cos) if rotary else None, _ptr(sin) if rotary else None,
+            _ptr(q_out), _ptr(k_out)), "kv_append_enqueue")
+
     def depth_unfold(self, x, y, taps, d_out, stride_d=1, pad_front=0, dil_d=1):
         """x [n, c, d, h, w] -> y [n * d_out, c * taps, h, w]: the depth taps of a 3-D convolution as channels."""
         n, c, d = x.shape[:3]
@@ -202,6 +237,165 @@ class Context:
         L.check(self._lib.sofie_b200_convert_enqueue(self._h, _ptr(x), _ptr(y), dtype_code(x.dtype),
                                                      dtype_code(y.dtype), rows, cols, _ptr(row_scale)),
                 "convert_enqueue")
+
+
+def _rows(name, t):
+    """(tokens, heads, head size, token pitch) of a [tokens, heads, head_dim] tensor whose rows may be column blocks of wider ones."""
+    if t.dim() != 3:
+        raise ValueError(f"{name}: [tokens, heads, head_dim] is expected, not {tuple(t.shape)}")
+    n, h, d = t.shape
+    sn, sh, sd = t.stride()
+    if (d > 1 and sd != 1) or (h > 1 and sh != d):
+        raise ValueError(f"{name}: the heads of a token must lie one behind another (strides {t.stride()})")
+    return n, h, d, sn if n > 1 else h * d
+
+
+def _same_rows(name, t, like):
+    """Token pitch of `t`, which has the shape and type of `like`."""
+    if t.shape != like.shape or t.dtype != like.dtype:
+        raise ValueError(f"{name}: {tuple(like.shape)} {like.dtype} is expected, not {tuple(t.shape)} {t.dtype}")
+    return _rows(name, t)[3]
+
+
+def _offsets(name, t, batch):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != batch + 1 or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 tensor of batch + 1 = {batch + 1} row offsets is expected")
+
+
+class PagedKV:
+    """A paged key-value cache and the sequences in it (sofie_b200_paged_kv): k and v [pages, page_size, kv_heads, head_dim] of
+    one shape and equal strides (innermost 1; a permuted or sliced view is fine), block_table int32 [batch, pages per sequence],
+    seq_lens int32 [batch] (lengths after the tokens of a pending append).  The object keeps the tensors; their contents may
+    change between calls (also under a captured graph), their places may not."""
+
+    def __init__(self, k, v, block_table, seq_lens):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+            raise ValueError("PagedKV: k and v are [pages, page_size, kv_heads, head_dim] of one shape, type and strides")
+        pages, page_size, kv_heads, dim = k.shape
+        if page_size < 1 or kv_heads < 1 or dim < 1 or (dim > 1 and k.stride(3) != 1):
+            raise ValueError("PagedKV: the head dimension must be the innermost, without gaps")
+        for name, t, rank in (("block_table", block_table, 2), ("seq_lens", seq_lens, 1)):
+            if t.dtype != torch.int32 or t.dim() != rank or (t.shape[-1] > 1 and t.stride(-1) != 1):
+                raise ValueError(f"PagedKV: {name} is an int32 tensor of rank {rank}, contiguous along its last axis")
+        if block_table.shape[0] != seq_lens.shape[0]:
+            raise ValueError("PagedKV: one row of the block table per sequence")
+        if len({t.device for t in (k, v, block_table, seq_lens)}) != 1:
+            raise ValueError("PagedKV: all tensors live on one device")
+        self.k, self.v, self.block_table, self.seq_lens = k, v, block_table, seq_lens
+        self.kv_heads, self.head_dim, self.dtype, self.batch = kv_heads, dim, k.dtype, seq_lens.shape[0]
+        width = block_table.shape[1]
+        # the stride of an axis of one element says nothing: the dense one stands for it
+        hs = k.stride(2) if kv_heads > 1 else dim
+        ts = k.stride(1) if page_size > 1 else max(hs, dim) * kv_heads
+        ps = k.stride(0) if pages > 1 else max(ts * page_size, hs * kv_heads)
+        self._desc = L.PagedKv(_ptr(k), _ptr(v), _ptr(block_table), _ptr(seq_lens), self.batch, pages, width,
+                               block_table.stride(0) if self.batch > 1 else width, ps, ts, hs, page_size)
+        self._ref = C.byref(self._desc)
+
+
+class PromptAttentionPlan:
+    """Attention over packed prompts (sofie_b200_prompt_attention_plan): causal or full, heads / kv_heads query heads per key head."""
+
+    def __init__(self, ctx: Context, heads, kv_heads, head_dim, dtype, causal=True, scale=0.0):
+        self.ctx, self._lib, self._dtype = ctx, ctx._lib, dtype
+        self._shape = (heads, kv_heads, head_dim)
+        self._desc = (heads, kv_heads, head_dim, dtype_code(dtype), int(causal), float(scale))
+        self._plans = {}
+        self._plan((0, 0, 0, 0))   # refuses at once what no pitch could mend
+
+    def _plan(self, pitches):
+        h = self._plans.get(pitches)
+        if h is None:
+            h = C.c_void_p()
+            d = L.PromptAttentionDesc(*self._desc, *pitches)
+            L.check(self._lib.sofie_b200_prompt_attention_plan_create(self.ctx._h, C.byref(d), C.byref(h)), "prompt_attention_plan_create")
+            self._plans[pitches] = h
+        return h
+
+    @property
+    def kernel(self) -> str:
+        return self._lib.sofie_b200_prompt_attention_plan_kernel(self._plan((0, 0, 0, 0))).decode()
+
+    def enqueue(self, q, k, v, y, cu_seqlens, cu_seqlens_k=None) -> None:
+        """q, y: [tokens, heads, head_dim]; k, v: [key tokens, kv_heads, head_dim], rows packed sequence behind sequence;
+        cu_seqlens (and cu_seqlens_k, where keys have other lengths than queries): int32 [batch + 1] row offsets."""
+        n, h, d, ldq = _rows("q", q)
+        nk, hk, dk, ldk = _rows("k", k)
+        if (h, hk, d) != self._shape or dk != d or q.dtype != self._dtype or k.dtype != self._dtype:
+            raise ValueError(f"prompt attention: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype} do not match the plan")
+        batch = cu_seqlens.shape[0] - 1
+        if batch < 0:
+            raise ValueError("cu_seqlens: batch + 1 row offsets are expected")
+        _offsets("cu_seqlens", cu_seqlens, batch)
+        if cu_seqlens_k is not None:
+            _offsets("cu_seqlens_k", cu_seqlens_k, batch)
+        pitches = (ldq, ldk, _same_rows("v", v, k), _same_rows("y", y, q))
+        L.check(self._lib.sofie_b200_prompt_attention_enqueue(self._plan(pitches), _ptr(q), _ptr(k), _ptr(v), _ptr(y), _ptr(cu_seqlens),
+                                                              _ptr(cu_seqlens_k), batch, n, nk), "prompt_attention_enqueue")
+
+    def close(self) -> None:
+        for h in self._plans.values():
+            self._lib.sofie_b200_prompt_attention_plan_destroy(h)
+        self._plans = {}
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class PagedAttentionPlan:
+    """Attention of one new token per sequence over a paged cache (sofie_b200_paged_attention_plan).  The plan owns the
+    workspace in which the parts of split sequences meet, so its calls belong on one stream, the context's; graphs that are
+    replayed side by side need a plan (and a context) each."""
+
+    def __init__(self, ctx: Context, heads, kv_heads, head_dim, dtype, scale=0.0):
+        self.ctx, self._lib, self._dtype = ctx, ctx._lib, dtype
+        self._shape = (heads, kv_heads, head_dim)
+        self._desc = (heads, kv_heads, head_dim, dtype_code(dtype), float(scale))
+        self._plans = {}
+        self._workspace = None
+        h = self._plan((0, 0))
+        size = int(self._lib.sofie_b200_paged_attention_workspace_bytes(h))
+        if size:
+            self._workspace = torch.empty(size, dtype=torch.uint8, device=f"cuda:{ctx.device}")
+            if ctx.stream is not None:   # freed memory must not be handed out again while the context's stream still uses it
+                self._workspace.record_stream(ctx.stream)
+
+    def _plan(self, pitches):
+        h = self._plans.get(pitches)
+        if h is None:
+            h = C.c_void_p()
+            d = L.PagedAttentionDesc(*self._desc, *pitches)
+            L.check(self._lib.sofie_b200_paged_attention_plan_create(self.ctx._h, C.byref(d), C.byref(h)), "paged_attention_plan_create")
+            self._plans[pitches] = h
+        return h
+
+    @property
+    def kernel(self) -> str:
+        return self._lib.sofie_b200_paged_attention_plan_kernel(self._plan((0, 0))).decode()
+
+    def enqueue(self, q, kv, y) -> None:
+        """q, y: [batch, heads, head_dim]; kv: the PagedKV with the cache and its batch of sequences."""
+        n, h, d, ldq = _rows("q", q)
+        if (h, kv.kv_heads, d) != self._shape or kv.head_dim != d or q.dtype != self._dtype or kv.dtype != self._dtype or n != kv.batch:
+            raise ValueError(f"paged attention: q {tuple(q.shape)} {q.dtype} over {kv.batch} sequences of {kv.kv_heads} heads of {kv.head_dim} "
+                             f"{kv.dtype} does not match the plan")
+        L.check(self._lib.sofie_b200_paged_attention_enqueue(self._plan((ldq, _same_rows("y", y, q))), _ptr(q), kv._ref, _ptr(y),
+                                                             _ptr(self._workspace)), "paged_attention_enqueue")
+
+    def close(self) -> None:
+        for h in self._plans.values():
+            self._lib.sofie_b200_paged_attention_plan_destroy(h)
+        self._plans = {}
+        self._workspace = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def make_epilogue(row_scale=None, col_scale=None, alpha=1.0, beta=1.0, bias=None, bias_mode=None, ldc=0,

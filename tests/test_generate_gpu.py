@@ -1,0 +1,549 @@
+"""The generation operators on the GPU against their statement in 64 bits (tests/generate_ref.py): appending to a paged
+cache with the rotation, attention over packed prompts, attention over the cache, and a run of the three together."""
+import math
+
+import pytest
+import torch
+
+import generate_ref as ref
+from sofie_b200 import lib as L
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture()
+def ctx(b200_lib):
+    from sofie_b200.ops import Context
+    c = Context(0)
+    yield c
+    c.close()
+
+
+def gen_of(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def normal(g, shape, dtype, std=1.0):
+    return (torch.randn(shape, generator=g, device=DEV) * std).to(dtype)
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def offsets(lens):
+    out = [0]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+def tables(positions, rotary):
+    r = rotary // 2
+    ang = torch.arange(positions, dtype=torch.float64, device=DEV)[:, None] * 10000.0 ** (-torch.arange(r, dtype=torch.float64, device=DEV) / max(r, 1))[None]
+    return ang.cos().float(), ang.sin().float()
+
+
+# ---- append ---------------------------------------------------------------------------------------------------------
+APPEND = [
+    # heads, kv_heads, dim, rotary, interleaved, page_size, [(past, new)], wide rows
+    (8, 8, 64, 64, False, 16, [(77, 1)], False),
+    (32, 8, 128, 128, False, 16, [(0, 5), (31, 1), (15, 17), (0, 0), (100, 33)], True),
+    (6, 2, 96, 48, True, 32, [(0, 40), (7, 100)], False),
+    (5, 1, 80, 40, False, 1, [(3, 9), (0, 1)], True),
+    (4, 4, 256, 256, True, 48, [(47, 2), (48, 50)], False),
+    (3, 3, 10, 6, False, 7, [(5, 20), (0, 3)], True),
+    (2, 1, 9, 2, True, 5, [(0, 11)], False),
+    (0, 4, 64, 0, False, 128, [(120, 20), (0, 256)], False),
+    (64, 1, 192, 96, False, 256, [(255, 1), (256, 1), (0, 1)], True),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(APPEND)))
+def test_append(ctx, case, dtype):
+    from sofie_b200.ops import PagedKV
+    heads, kvh, dim, rotary, inter, size, seqs, wide = APPEND[case]
+    g = gen_of(case)
+    new, lens = [n for _, n in seqs], [p + n for p, n in seqs]
+    cu = offsets(new)
+    rows = cu[-1] + 3   # three rows that belong to nobody
+    if wide:
+        allq = normal(g, (rows, heads + 2 * kvh, dim), dtype)
+        q, k, v = allq[:, :heads], allq[:, heads:heads + kvh], allq[:, heads + kvh:]
+    else:
+        q, k, v = normal(g, (rows, heads, dim), dtype), normal(g, (rows, kvh, dim), dtype), normal(g, (rows, kvh, dim), dtype)
+    table, pages = ref.make_pages(lens, size, g)
+    ck, cv = normal(g, (pages, size, kvh, dim), dtype), normal(g, (pages, size, kvh, dim), dtype)
+    want_k, want_v = ck.double(), cv.double()
+    tol_k = torch.zeros_like(want_k)
+    cos, sin = tables(max(lens) + 1, rotary)
+    pos = torch.tensor([p + i for p, n in seqs for i in range(n)], device=DEV, dtype=torch.long)
+    seq = torch.tensor([b for b, n in enumerate(new) for _ in range(n)], device=DEV, dtype=torch.long)
+    where, slot = table[seq, pos // size].long(), pos % size
+    zk, tk = ref.turn(k[:cu[-1]], pos, cos, sin, rotary, inter)
+    want_k[where, slot], tol_k[where, slot] = zk, tk
+    want_v[where, slot] = v[:cu[-1]].double()
+    q_out = torch.full((rows, heads, dim), 5.0, dtype=dtype, device=DEV) if heads else None
+    k_out = torch.full((rows, kvh, dim), 6.0, dtype=dtype, device=DEV)
+    kv = PagedKV(ck, cv, table, ints(lens))
+    ctx.kv_append(k, v, kv, ints(cu), cos=cos if rotary else None, sin=sin if rotary else None, interleaved=inter, q=q if heads else None,
+                  q_out=q_out, k_out=k_out)
+    ctx.sync()
+    ref.close(ck, want_k, tol_k, "cache k")
+    ref.close(cv, want_v, torch.zeros_like(want_v), "cache v")
+    ref.close(k_out[:cu[-1]], zk, tk, "k_out")
+    assert (k_out[cu[-1]:] == 6.0).all()
+    if heads:
+        zq, tq = ref.turn(q[:cu[-1]], pos, cos, sin, rotary, inter)
+        ref.close(q_out[:cu[-1]], zq, tq, "q_out")
+        assert (q_out[cu[-1]:] == 5.0).all()
+        # in place: the same bits
+        before = q_out.clone()
+        q2, k2 = q.contiguous().clone(), k.contiguous().clone()
+        ctx.kv_append(k2, v, kv, ints(cu), cos=cos if rotary else None, sin=sin if rotary else None, interleaved=inter, q=q2, q_out=q2, k_out=k2)
+        ctx.sync()
+        assert torch.equal(q2[:cu[-1]], before[:cu[-1]]) and torch.equal(k2[:cu[-1]], k_out[:cu[-1]])
+        assert torch.equal(q2[cu[-1]:], q[cu[-1]:]) and torch.equal(k2[cu[-1]:], k[cu[-1]:])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_append_one_token_each_with_padding_rows(ctx, dtype):
+    """No cu_seqlens: one token per sequence; rows of length 0 are padding and stay as they are.  Heads-first pages."""
+    from sofie_b200.ops import PagedKV
+    g = gen_of(3)
+    lens, size, heads, kvh, dim = [17, 0, 1, 64, 0], 16, 4, 2, 64
+    table, pages = ref.make_pages(lens, size, g)
+    ck, cv = (normal(g, (pages, kvh, size, dim), dtype).transpose(1, 2) for _ in range(2))
+    keep_k, keep_v = ck.clone(), cv.clone()
+    q, k, v = normal(g, (5, heads, dim), dtype), normal(g, (5, kvh, dim), dtype), normal(g, (5, kvh, dim), dtype)
+    cos, sin = tables(64, dim)
+    q_out = torch.full_like(q, 9.0)
+    ctx.kv_append(k, v, PagedKV(ck, cv, table, ints(lens)), cos=cos, sin=sin, q=q, q_out=q_out)
+    ctx.sync()
+    live = [0, 2, 3]
+    pos = torch.tensor([lens[b] - 1 for b in live], device=DEV)
+    zk, tk = ref.turn(k[live], pos, cos, sin, dim, False)
+    zq, tq = ref.turn(q[live], pos, cos, sin, dim, False)
+    ref.close(q_out[live], zq, tq)
+    assert (q_out[[1, 4]] == 9.0).all()
+    for i, b in enumerate(live):
+        p, s = int(table[b, (lens[b] - 1) // size]), (lens[b] - 1) % size
+        ref.close(ck[p, s], zk[i], tk[i])
+        assert torch.equal(cv[p, s], v[b])
+        ck[p, s], cv[p, s] = keep_k[p, s], keep_v[p, s]
+    assert torch.equal(ck, keep_k) and torch.equal(cv, keep_v)
+
+
+def test_append_leaves_out_bad_pages_and_positions(ctx):
+    """A page that does not exist, a position without a page or without an angle, a length smaller than the new tokens: those
+    tokens are left out, the others arrive, and the next sync says so once."""
+    from sofie_b200.ops import PagedKV
+    g = gen_of(4)
+    size, kvh, dim, pages = 4, 2, 32, 6
+    lens = [4, 8, 12, 1, 40, 4]
+    table = ints([[0, 0], [1, 99], [2, 3], [4, 4], [5, 5], [-7, 0]])
+    cu = offsets([1, 1, 1, 3, 1, 1])   # sequence 3 claims one token and brings three
+    ck, cv = normal(g, (pages, size, kvh, dim), BF), normal(g, (pages, size, kvh, dim), BF)
+    keep = ck.clone()
+    k, v = normal(g, (cu[-1], kvh, dim), BF), normal(g, (cu[-1], kvh, dim), BF)
+    cos, sin = tables(8, dim)   # sequence 2's token is at position 11
+    ctx.kv_append(k, v, PagedKV(ck, cv, table, ints(lens)), ints(cu), cos=cos, sin=sin)
+    with pytest.raises(L.SofieB200Error) as e:
+        ctx.sync()
+    assert e.value.status == L.ERR_DEVICE_INDEX
+    ctx.sync()
+    assert torch.equal(cv[0, 3], v[0]) and torch.equal(cv[4, 0], v[5])   # sequence 0, and the one token of sequence 3 that has a position
+    ck[0, 3], ck[4, 0] = keep[0, 3], keep[4, 0]
+    assert torch.equal(ck, keep)
+
+
+# ---- prompts --------------------------------------------------------------------------------------------------------
+PROMPT = [
+    # heads, kv_heads, dim, causal, query lengths, key lengths (None: the same)
+    (8, 8, 64, True, [40], None),
+    (8, 2, 64, True, [1, 127, 128, 129, 0, 255, 257, 2], None),
+    (8, 8, 128, True, [300, 1, 64, 65], None),
+    (32, 8, 128, True, [700, 33, 1], None),
+    (8, 8, 64, False, [128, 100, 24, 1], None),
+    (4, 4, 32, True, [200, 5], None),
+    (6, 2, 80, True, [77, 130], [200, 131]),
+    (7, 1, 96, False, [50, 19], [3, 400]),
+    (10, 2, 128, True, [60, 20, 9], [20, 20, 0]),
+    (16, 1, 64, True, [9, 300], [500, 300]),
+    (64, 1, 128, True, [3, 130], None),
+    (4, 1, 256, True, [150, 31], [300, 31]),
+    (3, 3, 192, False, [140], [129]),
+    (5, 1, 8, True, [13, 260], None),
+    (2, 2, 104, True, [129], [513]),
+    (12, 1, 128, True, [1] * 40, [5] * 40),
+    (8, 2, 128, True, [1200], [2048]),
+]
+
+
+def prompt_case(heads, kvh, dim, lq, lk, dtype, seed, spare=5, wide=False):
+    g = gen_of(seed)
+    cq, ck = offsets(lq), offsets(lk or lq)
+    n, m = cq[-1] + spare, ck[-1] + spare
+    if wide and lk is None:
+        allq = normal(g, (n, heads + 2 * kvh, dim), dtype)
+        q, k, v = allq[:, :heads], allq[:, heads:heads + kvh], allq[:, heads + kvh:]
+        q.mul_(1.5)
+    else:
+        q, k, v = normal(g, (n, heads, dim), dtype, 1.5), normal(g, (m, kvh, dim), dtype), normal(g, (m, kvh, dim), dtype)
+    return q, k, v, cq, ck
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(PROMPT)))
+def test_prompt(ctx, case, dtype):
+    from sofie_b200.ops import PromptAttentionPlan
+    heads, kvh, dim, causal, lq, lk = PROMPT[case]
+    q, k, v, cq, ck = prompt_case(heads, kvh, dim, lq, lk, dtype, case, wide=case % 2 == 1)
+    want, tol = ref.prompt(q, k, v, cq, ck, causal)
+    for t, end in ((q, cq[-1]), (k, ck[-1]), (v, ck[-1])):
+        t[end:] = float("nan")          # rows behind the last sequence hold anything
+    y = torch.full((q.shape[0], heads, dim), 3.0, dtype=dtype, device=DEV)
+    plan = PromptAttentionPlan(ctx, heads, kvh, dim, dtype, causal=causal)
+    plan.enqueue(q, k, v, y, ints(cq), ints(ck) if lk else None)
+    ctx.sync()
+    ref.close(y[:cq[-1]], want[:cq[-1]], tol[:cq[-1]], plan.kernel)
+    assert (y[cq[-1]:] == 3.0).all()
+    again = torch.empty_like(y)
+    plan.enqueue(q, k, v, again, ints(cq), ints(ck) if lk else None)
+    ctx.sync()
+    assert torch.equal(again[:cq[-1]], y[:cq[-1]])
+    plan.close()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("heads,kvh,dim", [(4, 1, 64), (2, 2, 128)])
+def test_prompt_hidden_keys_have_no_influence(ctx, dtype, heads, kvh, dim):
+    """NaN and infinities in keys and values that a query does not see: the next sequence's, and later ones of its own."""
+    from sofie_b200.ops import PromptAttentionPlan
+    lens = [130, 70, 20]
+    q, k, v, cq, _ = prompt_case(heads, kvh, dim, lens, None, dtype, 11)
+    k[130:200] = float("nan")            # the whole second sequence
+    v[130:200] = float("inf")
+    k[100], v[90] = float("nan"), float("-inf")     # late tokens of the first
+    v[215, :, 3] = float("nan")
+    y = torch.zeros_like(q)
+    PromptAttentionPlan(ctx, heads, kvh, dim, dtype).enqueue(q, k, v, y, ints(cq))
+    ctx.sync()
+    want, tol = ref.prompt(q, k, v, cq, cq, True)
+    # the statement in 64 bits computes 0 * NaN; put those rows right: they see only what comes before
+    for s, e, first in ((0, 130, 90), (200, 220, 215)):
+        w2, t2 = ref.prompt(q[s:first], k[s:first], v[s:first], [0, first - s], [0, first - s], True)
+        ref.close(y[s:first], w2, t2, f"rows {s}..{first}")
+    assert torch.isnan(y[100:130]).all()
+    late = v[90].double().sign() * math.inf
+    assert (y[90:100].double() == late[0, 0]).all()
+    assert torch.isnan(y[215:220, :, 3]).all() and torch.isfinite(y[215:220, :, :3]).all()
+
+
+def test_prompt_rows_far_from_the_maximum(ctx):
+    """Scores that grow along the keys by more than fp32's exponents hold: the running maximum has to follow."""
+    from sofie_b200.ops import PromptAttentionPlan
+    for dtype in (BF, F32):
+        n, dim = 520, 64
+        g = gen_of(5)
+        q, k, v = normal(g, (n, 1, dim), dtype, 0.1), normal(g, (n, 1, dim), dtype, 0.1), normal(g, (n, 1, dim), dtype)
+        q[:, 0, 0] = 8.0
+        k[:, 0, 0] = (torch.arange(n, device=DEV) * 0.5).to(dtype)       # scores 0 .. 260
+        k[300:, 0, 0] = -(torch.arange(n - 300, device=DEV) * 1.0).to(dtype)
+        y = torch.zeros_like(q)
+        for causal in (True, False):
+            PromptAttentionPlan(ctx, 1, 1, dim, dtype, causal=causal).enqueue(q, k, v, y, ints([0, n]))
+            ctx.sync()
+            ref.close(y, *ref.prompt(q, k, v, [0, n], [0, n], causal))
+
+
+def test_prompt_bad_offsets_are_left_out(ctx):
+    from sofie_b200.ops import PromptAttentionPlan
+    for dtype in (BF, F32):
+        q, k, v, cq, _ = prompt_case(4, 2, 64, [20, 30], None, dtype, 6, spare=0)
+        want, tol = ref.prompt(q, k, v, cq, cq, True)
+        plan = PromptAttentionPlan(ctx, 4, 2, 64, dtype)
+        y = torch.full_like(q, 3.0)
+        plan.enqueue(q, k, v, y, ints(cq), ints([0, 20, 60]))      # ten keys too many for the second sequence
+        with pytest.raises(L.SofieB200Error) as e:
+            ctx.sync()
+        assert e.value.status == L.ERR_DEVICE_INDEX
+        ref.close(y[:20], want[:20], tol[:20])
+        assert (y[20:] == 3.0).all()
+        for cu in ([0, 30, 20], [-5, 20, 50], [0, 2000000000, 50], [0, 20, 51]):
+            plan.enqueue(q, k, v, y, ints(cu))
+            try:
+                ctx.sync()
+            except L.SofieB200Error as err:
+                assert err.status == L.ERR_DEVICE_INDEX
+
+
+def test_prompt_far_rows(ctx):
+    """Element offsets past 2^31: a token pitch of 2^23 elements."""
+    from sofie_b200.ops import PromptAttentionPlan
+    n, pitch = 280, 1 << 23
+    buf = torch.empty(n * pitch, dtype=BF, device=DEV)
+    rows = buf.view(n, pitch)
+    g = gen_of(8)
+    for dim, col in ((64, 0),):
+        q, k, v, y = (rows[:, c:c + 2 * dim].view(n, 2, dim) for c in (0, 2 * dim, 4 * dim, 6 * dim))
+        for t in (q, k, v):
+            t.copy_(normal(g, t.shape, BF))
+        PromptAttentionPlan(ctx, 2, 2, dim, BF).enqueue(q, k, v, y, ints([0, n]))
+        ctx.sync()
+        ref.close(y, *ref.prompt(q, k, v, [0, n], [0, n], True))
+
+
+# ---- decode ---------------------------------------------------------------------------------------------------------
+DECODE = [
+    # heads, kv_heads, dim, page_size, lengths, pages heads first
+    (8, 8, 64, 16, [5, 1, 0, 16, 17, 100], False),
+    (32, 8, 128, 16, [1000, 3, 64, 63, 65], False),
+    (32, 8, 128, 64, [5000], False),
+    (8, 2, 64, 1, [300, 40], False),
+    (6, 2, 80, 48, [500, 47, 48, 49], True),
+    (7, 1, 96, 128, [1, 2, 127, 128, 129, 1000], False),
+    (16, 1, 128, 32, [777, 31], True),
+    (64, 1, 128, 16, [900, 1], False),
+    (20, 1, 64, 16, [333, 2048], False),
+    (4, 1, 256, 8, [600, 9], False),
+    (5, 5, 32, 256, [1, 255, 256, 257, 2000], False),
+    (3, 1, 8, 16, [100] * 70, False),
+    (12, 4, 192, 16, [129] * 9 + [0] * 5, True),
+    (1, 1, 128, 16, [40000], False),
+    (8, 8, 64, 16, [13] * 300, False),
+]
+
+
+def decode_case(heads, kvh, dim, size, lens, first, dtype, seed):
+    g = gen_of(seed)
+    table, pages = ref.make_pages(lens, size, g)
+    if first:
+        ck, cv = (normal(g, (pages, kvh, size, dim), dtype).transpose(1, 2) for _ in range(2))
+    else:
+        both = normal(g, (pages, 2, size, kvh, dim), dtype)
+        ck, cv = both[:, 0], both[:, 1]
+    return normal(g, (len(lens), heads, dim), dtype, 1.5), ck, cv, table
+
+
+def poison(cache, table, lens, size):
+    """NaN in every slot that no sequence owns."""
+    keep = torch.zeros(cache.shape[:2], dtype=torch.bool, device=DEV)
+    for b, n in enumerate(lens):
+        at = torch.arange(n, device=DEV)
+        keep[table[b, at // size].long(), at % size] = True
+    cache[~keep] = float("nan")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("case", range(len(DECODE)))
+def test_decode(ctx, case, dtype):
+    from sofie_b200.ops import PagedAttentionPlan, PagedKV
+    heads, kvh, dim, size, lens, first = DECODE[case]
+    q, ck, cv, table = decode_case(heads, kvh, dim, size, lens, first, dtype, case)
+    want, tol = ref.decode(q, ck, cv, table, lens)
+    poison(ck, table, lens, size)
+    poison(cv, table, lens, size)
+    y = torch.full_like(q, 3.0)
+    plan = PagedAttentionPlan(ctx, heads, kvh, dim, dtype)
+    kv = PagedKV(ck, cv, table, ints(lens))
+    plan.enqueue(q, kv, y)
+    ctx.sync()
+    ref.close(y, want, tol, plan.kernel)
+    again = torch.empty_like(y)
+    plan.enqueue(q, kv, again)
+    ctx.sync()
+    assert torch.equal(again, y)
+    plan.close()
+
+
+def test_decode_leaves_out_bad_pages(ctx):
+    from sofie_b200.ops import PagedAttentionPlan, PagedKV
+    for dtype in (BF, F32):
+        lens, size = [40, 40, 40, 40], 16
+        q, ck, cv, table = decode_case(4, 2, 64, size, lens, False, dtype, 21)
+        want, tol = ref.decode(q, ck, cv, table, [40, 32, 40, 48])
+        n_pages = ck.shape[0]
+        table[1, 2] = n_pages                              # sequence 1 loses its last 8 tokens
+        kv = PagedKV(ck, cv, table, ints([40, 40, -3, 4000]))   # sequence 2: a negative length; 3: more than its table holds
+        y = torch.full_like(q, 3.0)
+        plan = PagedAttentionPlan(ctx, 4, 2, 64, dtype)
+        plan.enqueue(q, kv, y)
+        with pytest.raises(L.SofieB200Error) as e:
+            ctx.sync()
+        assert e.value.status == L.ERR_DEVICE_INDEX
+        ref.close(y[:2], want[:2], tol[:2])
+        assert (y[2] == 0).all()
+        ref.close(y[3], want[3], tol[3])
+        table[0] = -1                                      # no page at all: nothing to attend to
+        plan.enqueue(q, kv, y)
+        with pytest.raises(L.SofieB200Error):
+            ctx.sync()
+        assert (y[0] == 0).all()
+
+
+def test_far_pages(ctx):
+    """Cache offsets past 2^31 elements: append there and read it back."""
+    from sofie_b200.ops import PagedAttentionPlan, PagedKV
+    kvh, dim, size = 2, 64, 16
+    pages = (1 << 31) // (kvh * dim * size) + 40
+    g = gen_of(9)
+    ck, cv = (torch.empty((pages, size, kvh, dim), dtype=BF, device=DEV) for _ in range(2))
+    table = ints([[pages - 1, pages - 3, 0], [pages - 2, 1, pages - 5]])
+    lens = [40, 48]
+    k, v, q = normal(g, (88, kvh, dim), BF), normal(g, (88, kvh, dim), BF), normal(g, (2, 4, dim), BF)
+    kv = PagedKV(ck, cv, table, ints(lens))
+    ctx.kv_append(k, v, kv, ints([0, 40, 88]))
+    y = torch.zeros_like(q)
+    PagedAttentionPlan(ctx, 4, kvh, dim, BF).enqueue(q, kv, y)
+    ctx.sync()
+    assert torch.equal(ref.gather(ck, table[0], 40), k[:40]) and torch.equal(ref.gather(cv, table[1], 48), v[40:])
+    ref.close(y, *ref.decode(q, ck, cv, table, lens))
+
+
+# ---- together -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,heads,kvh,dim", [(BF, 8, 2, 64), (F32, 4, 4, 32), (BF, 8, 8, 128)], ids=["bf16-grouped", "f32", "bf16-128"])
+def test_generation_run(ctx, dtype, heads, kvh, dim):
+    """Prompts enter the cache (append + prompt attention over the rotated keys), then tokens are generated one by one (append +
+    attention over the cache).  Every step's result is the causal attention of the whole sequence so far, in 64 bits."""
+    from sofie_b200.ops import PagedAttentionPlan, PagedKV, PromptAttentionPlan
+    g = gen_of(31)
+    prompts, steps, size = [70, 1, 133], 20, 16
+    total = [n + steps for n in prompts]
+    table, pages = ref.make_pages(total, size, g)
+    ck, cv = (torch.full((pages, size, kvh, dim), float("nan"), dtype=dtype, device=DEV) for _ in range(2))
+    lens = ints(prompts)
+    kv = PagedKV(ck, cv, table, lens)
+    cos, sin = tables(max(total), dim)
+    cu = offsets(prompts)
+    qkv = normal(g, (cu[-1], heads + 2 * kvh, dim), dtype)
+    q, k, v = qkv[:, :heads], qkv[:, heads:heads + kvh], qkv[:, heads + kvh:]
+    qr, kr, y = torch.empty((cu[-1], heads, dim), dtype=dtype, device=DEV), torch.empty((cu[-1], kvh, dim), dtype=dtype, device=DEV), torch.empty((cu[-1], heads, dim), dtype=dtype, device=DEV)
+    prompt, step = PromptAttentionPlan(ctx, heads, kvh, dim, dtype), PagedAttentionPlan(ctx, heads, kvh, dim, dtype)
+    ctx.kv_append(k, v, kv, ints(cu), cos=cos, sin=sin, q=q, q_out=qr, k_out=kr)
+    prompt.enqueue(qr, kr, v, y, ints(cu))
+    ctx.sync()
+    ref.close(y, *ref.prompt(qr, kr, v, cu, cu, True), "prompts")
+    for b, n in enumerate(prompts):
+        assert torch.equal(ref.gather(ck, table[b], n), kr[cu[b]:cu[b + 1]])
+    ys = torch.empty((3, heads, dim), dtype=dtype, device=DEV)
+    for i in range(steps):
+        lens += 1
+        qkv = normal(g, (3, heads + 2 * kvh, dim), dtype)
+        q1 = torch.empty((3, heads, dim), dtype=dtype, device=DEV)
+        ctx.kv_append(qkv[:, heads:heads + kvh], qkv[:, heads + kvh:], kv, cos=cos, sin=sin, q=qkv[:, :heads], q_out=q1)
+        step.enqueue(q1, kv, ys)
+        ctx.sync()
+        ref.close(ys, *ref.decode(q1, ck, cv, table, [n + i + 1 for n in prompts]), f"step {i}")
+    # the last step once more as the last row of a causal prompt over the whole sequence
+    full = [ref.gather(ck, table[b], n) for b, n in enumerate(total)], [ref.gather(cv, table[b], n) for b, n in enumerate(total)]
+    y1 = torch.empty_like(ys)
+    prompt.enqueue(q1, torch.cat(full[0]), torch.cat(full[1]), y1, ints([0, 1, 2, 3]), ints(offsets(total)))
+    ctx.sync()
+    w, t = ref.decode(q1, ck, cv, table, total)
+    ref.close(y1, w, t + 2.0 ** -8 * (w.abs() + 4.0 * (dtype == BF)), "last step as a prompt")
+
+
+def test_a_captured_step_is_replayed_for_other_lengths(b200_lib):
+    """Append and attention of one step captured into a graph, replayed while the lengths and inputs change in place."""
+    from sofie_b200.ops import Context, PagedAttentionPlan, PagedKV, PromptAttentionPlan
+    side = torch.cuda.Stream(device=DEV)
+    ctx = Context(0, stream=side)
+    g = gen_of(41)
+    heads, kvh, dim, size, room = 8, 2, 128, 16, 700
+    table, pages = ref.make_pages([room] * 4, size, g)
+    ck, cv = normal(g, (pages, size, kvh, dim), BF), normal(g, (pages, size, kvh, dim), BF)
+    lens = ints([1, 1, 1, 1])
+    kv = PagedKV(ck, cv, table, lens)
+    cos, sin = tables(room, dim)
+    q, k, v = normal(g, (4, heads, dim), BF), normal(g, (4, kvh, dim), BF), normal(g, (4, kvh, dim), BF)
+    qr, y, yp = torch.empty_like(q), torch.empty_like(q), torch.zeros_like(q)
+    plan, prompt = PagedAttentionPlan(ctx, heads, kvh, dim, BF), PromptAttentionPlan(ctx, heads, kvh, dim, BF)
+    cu = ints([0, 2, 3, 4, 4])
+
+    def step():
+        ctx.kv_append(k, v, kv, cos=cos, sin=sin, q=q, q_out=qr)
+        plan.enqueue(qr, kv, y)
+        prompt.enqueue(q, k, v, yp, cu)
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step()
+    ctx.sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for i, now in enumerate(([5, 700, 0, 64], [699, 1, 333, 2], [1, 2, 3, 4])):
+        lens.copy_(ints(now))
+        q.copy_(normal(g, q.shape, BF))
+        k.copy_(normal(g, k.shape, BF))
+        cu.copy_(ints([[0, 2, 3, 4, 4], [0, 4, 4, 4, 4], [0, 1, 2, 3, 4]][i]))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        ctx.sync()
+        w, t = ref.decode(qr, ck, cv, table, now)
+        live = [b for b, n in enumerate(now) if n]
+        ref.close(y[live], w[live], t[live], f"replay {i}")
+        assert (y[[b for b, n in enumerate(now) if not n]] == 0).all()
+        c = cu.tolist()
+        ref.close(yp, *ref.prompt(q, k, v, c, c, True), f"replay {i}, prompt")
+    del graph
+    plan.close()
+    prompt.close()
+    ctx.close()
+
+
+def test_two_streams_at_once(b200_lib):
+    """Two contexts with plans of their own on two streams, their calls interleaved."""
+    from sofie_b200.ops import Context, PagedAttentionPlan, PagedKV
+    streams = [torch.cuda.Stream(device=DEV) for _ in range(2)]
+    runs = []
+    for i, s in enumerate(streams):
+        c = Context(0, stream=s)
+        lens = [3000 + i, 17, 900]
+        q, ck, cv, table = decode_case(16, 4, 128, 16, lens, False, BF, 50 + i)
+        runs.append((c, PagedAttentionPlan(c, 16, 4, 128, BF), q, PagedKV(ck, cv, table, ints(lens)), torch.empty_like(q), ref.decode(q, ck, cv, table, lens)))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, plan, q, kv, y, _w in runs:
+            plan.enqueue(q, kv, y)
+    for c, plan, q, kv, y, (want, tol) in runs:
+        c.sync()
+        ref.close(y, want, tol)
+        plan.close()
+        c.close()
+
+
+def test_refusals_with_a_context(ctx):
+    from sofie_b200.ops import PagedAttentionPlan, PagedKV, PromptAttentionPlan
+    q, ck, cv, table = decode_case(4, 2, 64, 16, [20, 20], False, BF, 1)
+    kv = PagedKV(ck, cv, table, ints([20, 20]))
+    plan = PagedAttentionPlan(ctx, 4, 2, 64, BF)
+    with pytest.raises(ValueError):
+        plan.enqueue(q[:1], kv, torch.empty_like(q[:1]))
+    with pytest.raises(ValueError):
+        plan.enqueue(q.float(), kv, torch.empty_like(q).float())
+    odd = torch.empty(2 * 4 * 64 + 1, dtype=BF, device=DEV)[1:].view(2, 4, 64)
+    with pytest.raises(L.SofieB200Error, match="aligned"):
+        plan.enqueue(odd, kv, torch.empty_like(q))
+    wide = torch.empty((2, 4 * 64 + 4), dtype=BF, device=DEV)[:, :256].view(2, 4, 64)
+    with pytest.raises(L.SofieB200Error, match="multiples of 8"):
+        plan.enqueue(wide, kv, torch.empty_like(q))
+    prompt = PromptAttentionPlan(ctx, 4, 2, 64, BF)
+    k = torch.empty((2, 2, 64), dtype=BF, device=DEV)
+    with pytest.raises(L.SofieB200Error, match="aligned"):
+        prompt.enqueue(odd, k, k, torch.empty_like(q), ints([0, 2]))
+    with pytest.raises(ValueError):
+        prompt.enqueue(q, k, k, q.float(), ints([0, 2]))
+    with pytest.raises(ValueError):
+        prompt.enqueue(q, k, k, q, ints([0, 2]).long())
+    with pytest.raises(L.SofieB200Error, match="head size"):
+        PromptAttentionPlan(ctx, 4, 2, 68, BF)
+    prompt.enqueue(q[:0], k, k, q[:0], ints([0]))     # nothing to do is not an error
+    ctx.sync()
