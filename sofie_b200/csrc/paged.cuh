@@ -65,4 +65,31 @@ SB_HD int packed_find(const int32_t *cu, int batch, int t) {
   return batch > 0 && cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
 }
 
+// ---- attention over the cache: dealing the work of a batch to blocks --------------------------------------------------
+// The work is a row of equal units (`unit` keys of one key head of one sequence), ordered by sequence, then head, then key; block c of
+// `blocks` takes the units [split_at(U, blocks, c), split_at(U, blocks, c + 1)).  Shares differ by one unit at most, whatever
+// the lengths are.  A part of an item (one head of one sequence) that is not the whole of it goes to a slot of the workspace:
+// slot 0 of its block when the item began in an earlier block, slot 1 when it begins here and goes on.  A block has at most one of each.
+SB_HD long long split_at(long long units, int blocks, int c) { return units / blocks * c + units % blocks * c / blocks; }
+
+// The last block that holds a unit before `end`, 0 < end <= units.
+SB_HD int split_last(long long units, int blocks, long long end) {
+  int lo = 0, hi = blocks - 1;   // the largest c with split_at(c) < end
+  while (lo < hi) {
+    const int mid = lo + (hi - lo + 1) / 2;
+    if (split_at(units, blocks, mid) < end) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Blocks that get work: no block fewer than `least` units, unless there are fewer in all.
+SB_HD int split_blocks(long long units, int blocks, int least) {
+  const long long most = (units + least - 1) / least;
+  return most < 1 ? 1 : most < blocks ? (int)most : blocks;
+}
+
+// Units of a sequence of n tokens.
+SB_HD int units_of(int n, int unit) { return (int)(((long long)n + unit - 1) / unit); }
+
 }  // namespace sb200

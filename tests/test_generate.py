@@ -219,3 +219,73 @@ def build_and_run(tmp_path, source):
 
 def test_index_arithmetic_over_hostile_tables(tmp_path):
     build_and_run(tmp_path, HOSTILE)
+
+
+SPLIT = r'''
+#include "paged.cuh"
+#include <algorithm>
+#include <cstdio>
+#include <vector>
+using namespace sb200;
+#define NEED(c) do { if (!(c)) { printf("failed: %s (line %d)\n", #c, __LINE__); return 1; } } while (0)
+static unsigned rs = 99;
+static int rnd(int n) { rs = rs * 1664525u + 1013904223u; return (int)((rs >> 8) % (unsigned)n); }
+int main() {
+  for (int it = 0; it < 4000; ++it) {
+    const int batch = 1 + rnd(12), items = 1 + rnd(9), unit = rnd(2) ? 64 : 32, grid = 1 + rnd(it % 2 ? 30 : 600), least = 1 + rnd(4);
+    std::vector<int> n(batch);
+    for (auto &x : n) x = rnd(4) ? rnd(it % 3 ? 700 : 9000) : rnd(2);
+    long long units = 0;
+    std::vector<long long> end;   // of each item in the row of units
+    for (int b = 0; b < batch; ++b)
+      for (int i = 0; i < items && n[b]; ++i) end.push_back(units += units_of(n[b], unit));
+    const int blocks = split_blocks(units, grid, least);
+    NEED(blocks >= 1 && blocks <= grid);
+    NEED(blocks == 1 || units / blocks >= 1);
+    std::vector<int> parts(end.size()), whole(end.size());
+    long long at = 0, lo = 1LL << 60, hi = 0;
+    for (int c = 0; c < blocks; ++c) {
+      const long long b = split_at(units, blocks, c), e = split_at(units, blocks, c + 1);
+      NEED(b == at && e >= b);
+      at = e;
+      lo = std::min(lo, e - b);
+      hi = std::max(hi, e - b);
+      int slot0 = 0, slot1 = 0;
+      for (size_t i = 0; i < end.size(); ++i) {
+        const long long first = i ? end[i - 1] : 0, s = std::max(b, first), t = std::min(e, end[i]);
+        if (s >= t) continue;
+        if (s == first && t == end[i]) { ++whole[i]; continue; }
+        ++parts[i];
+        if (s == first) {
+          ++slot1;
+          const int last = split_last(units, blocks, end[i]);
+          NEED(last > c && last < blocks);
+          NEED(split_at(units, blocks, last) < end[i] && split_at(units, blocks, last + 1) >= end[i]);
+        } else {
+          ++slot0;
+        }
+      }
+      NEED(slot0 <= 1 && slot1 <= 1);
+    }
+    NEED(at == units && (units == 0 || hi - lo <= 1));
+    for (size_t i = 0; i < end.size(); ++i) {
+      const long long first = i ? end[i - 1] : 0;
+      NEED((whole[i] == 1 && parts[i] == 0) || (whole[i] == 0 && parts[i] >= 2));
+      if (parts[i]) {   // the parts are those of consecutive blocks, as the joining kernel takes them
+        int c0 = 0;
+        while (split_at(units, blocks, c0 + 1) <= first) ++c0;
+        NEED(split_last(units, blocks, end[i]) - c0 + 1 == parts[i]);
+      }
+    }
+  }
+  // far: 2^31 - 1 tokens in each of 2^20 sequences
+  const long long units = (1LL << 20) * units_of(2147483647, 32) * 64;
+  NEED(units_of(2147483647, 32) == 1 << 26 && split_at(units, 296, 296) == units && split_at(units, 296, 0) == 0 && split_last(units, 296, units) == 295);
+  puts("ok");
+  return 0;
+}
+'''
+
+
+def test_dealing_of_units_to_blocks(tmp_path):
+    build_and_run(tmp_path, SPLIT)
