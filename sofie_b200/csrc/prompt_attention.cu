@@ -148,6 +148,12 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptParams p) 
   }
 }
 
+// A wait of a whole warp.  The lanes leave together: one that lagged behind could find the barrier a phase further on, with the parity
+// that means "not yet", and wait for good; and all of them agree on a wait that ran out.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
 // ---- bf16 on the tensor cores --------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -162,31 +168,50 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
       "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t *r) {
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t *r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-constexpr int PU_THREADS = 192;   // warps 0-3: a row of the tile per thread; warp 4: TMA; warp 5: MMA
-constexpr int PU_KEYS = 128;      // keys of a tile
-
+// A block computes TILES tiles of 128 rows against the same keys and values.  What sets the sizes is the way from L2: a tile of keys
+// and values takes about 3000 cycles from request to arrival and an SM sustains about 48 bytes per cycle, while the tensor cores
+// would finish 128 rows x 128 keys of head size 128 (64 KB of keys and values) in 1024 cycles.  So at that head size two tiles of rows
+// share every load (32 bytes per cycle at full rate) and five tiles of keys or values are in flight; at head size 64 half the bytes
+// are needed per score, and two blocks of one tile share an SM instead, one's beginning and end beside the other's middle.
 template <int DP>
-struct UmmaCfg {
-  static constexpr int PANELS = DP / 64;                   // a panel: 128 rows x 64 elements, 128-byte swizzle
-  static constexpr int TILE = PANELS * 16384;              // Q, or one tile of K or V
-  static constexpr int STAGES = DP == 64 ? 2 : 1;          // tiles of K (and of V) in flight
-  static constexpr int SMEM = (1 + 2 * STAGES) * TILE + 1024 /*barriers*/ + 1024 /*alignment*/;
-  static constexpr int O_COL = 128;                        // tensor memory: scores in columns 0 .. 127, the result from here
-  static constexpr int COLS = DP <= 128 ? 256 : 512;
-  static constexpr bool EARLY = DP == 64;                  // the weights have columns of their own: scores of the next tile meanwhile
-  static constexpr int P_COL = EARLY ? 192 : 0;
+struct UmmaCfg;
+template <>
+struct UmmaCfg<64> {
+  static constexpr int TILES = 1, KEYS = 128, BLOCKS = 2, STAGES = 5, COLS = 256;
+  static constexpr int S_COL = 0, O_COL = 128, P_COL = 192, STEP = 0;
+  static constexpr bool EARLY = true;    // the weights have columns of their own: the next scores are computed meanwhile
+  static constexpr bool HOLD = false;    // a thread holds its whole row of scores in registers
+};
+template <>
+struct UmmaCfg<128> {
+  static constexpr int TILES = 2, KEYS = 128, BLOCKS = 1, STAGES = 5, COLS = 512;
+  static constexpr int S_COL = 0, O_COL = 128, P_COL = 0, STEP = 256;
+  static constexpr bool EARLY = false, HOLD = true;
+};
+template <>
+struct UmmaCfg<256> {
+  static constexpr int TILES = 1, KEYS = 64, BLOCKS = 1, STAGES = 5, COLS = 512;
+  static constexpr int S_COL = 0, O_COL = 256, P_COL = 64, STEP = 0;
+  static constexpr bool EARLY = true, HOLD = true;
+};
+template <int DP>
+struct UmmaSize : UmmaCfg<DP> {
+  using C = UmmaCfg<DP>;
+  static constexpr int PANELS = DP / 64;                    // a panel: rows x 64 elements, 128-byte swizzle
+  static constexpr int Q = C::TILES * PANELS * 16384;
+  static constexpr int TILE = C::KEYS * DP * 2;             // keys or values
+  static constexpr int PANEL = C::KEYS * 128;
+  static constexpr int THREADS = C::TILES * 128 + 64;       // warps of rows; then TMA, MMA
+  static constexpr int SMEM = Q + C::STAGES * TILE + 1024 /*barriers*/ + 1024 /*alignment*/;
 };
 
 // The plain sum for one row, from global memory.  Taken when values that some rows of a tile do not see hold NaN or infinities: the
@@ -218,62 +243,65 @@ __device__ __noinline__ void plain_row(const PromptParams &p, long long q_row, i
   }
 }
 
-// A block computes one tile of 128 rows; two blocks share an SM (head sizes up to 128), so that one's softmax runs beside the other's
-// tensor-core work, and its beginning and end beside the other's middle.
-//   warp 4, lane 0   TMA: the queries once, then per tile of 128 keys K and V, from the last tile to the first
-//   warp 5, lane 0   MMA: S = Q K^T (operands in shared memory), O += P V (P in tensor memory, V MN-major in shared memory)
-//   warps 0-3        a thread per row: maximum, exponentials, row sum; P as bf16 back to tensor memory, over S's columns
+// Roles:
+//   a warp, lane 0   TMA: the queries once, then per tile of keys K and V, from the last tile to the first, into a ring
+//   a warp           MMA: S = Q K^T (operands in shared memory), O += P V (P in tensor memory, V MN-major in shared memory)
+//   4 warps a tile   a thread per row: maximum, exponentials, row sum; P as bf16 back to tensor memory
 // The reference maximum of a row moves only when a tile's maximum is 2^8 above it (weights stay below 2^8, exact in effect
 // since numerator and denominator use the same); then O is rescaled in tensor memory, which after the first tiles is rare.
 // Only tiles that the sequence's end or the diagonal cross pay for masks.
 template <int DP>
-__global__ void __launch_bounds__(PU_THREADS, DP <= 128 ? 2 : 1)
+__global__ void __launch_bounds__(UmmaSize<DP>::THREADS, UmmaSize<DP>::BLOCKS)
 prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const __grid_constant__ PromptParams p) {
-  using Cfg = UmmaCfg<DP>;
-  constexpr int ST = Cfg::STAGES;
+  using Cfg = UmmaSize<DP>;
+  constexpr int ST = Cfg::STAGES, KEYS = Cfg::KEYS, TILES = Cfg::TILES;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), pad = (1024u - (raw & 1023u)) & 1023u;
-  const uint32_t sm_q = raw + pad, sm_kv = sm_q + Cfg::TILE;   // [stage][K | V]
+  const uint32_t sm_q = raw + pad, sm_ring = sm_q + Cfg::Q;
   uint8_t *gen = smem_raw + pad;
-  uint8_t *tail = gen + (1 + 2 * ST) * Cfg::TILE;
+  uint8_t *tail = gen + Cfg::Q + ST * Cfg::TILE;
   const uint32_t bar_q = smem_u32(tail);             // queries landed
-  const uint32_t bar_kf = bar_q + 8;                 // [ST] keys landed
-  const uint32_t bar_ke = bar_kf + 8 * ST;           // [ST] keys read
-  const uint32_t bar_vf = bar_ke + 8 * ST;           // [ST] values landed
-  const uint32_t bar_ve = bar_vf + 8 * ST;           // [ST] values read (the product of the tile is complete)
-  const uint32_t bar_s = bar_ve + 8 * ST;            // scores complete in tensor memory
-  const uint32_t bar_se = bar_s + 8;                 // scores read (EARLY)
-  const uint32_t bar_p = bar_se + 8;                 // weights written to tensor memory
-  const uint32_t bar_o = bar_p + 8;                  // result complete
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 256);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + 260);
-  volatile int *unclean = reinterpret_cast<volatile int *>(tail + 264);   // non-finite values where the mask hides some of them
+  const uint32_t bar_full = bar_q + 8;               // [ST] ring: keys or values landed
+  const uint32_t bar_empty = bar_full + 8 * ST;      // [ST] the products that read them are complete
+  const uint32_t bar_s = bar_empty + 8 * ST;         // [TILES] scores complete in tensor memory
+  const uint32_t bar_se = bar_s + 8 * TILES;         // [TILES] scores read (EARLY)
+  const uint32_t bar_p = bar_se + 8 * TILES;         // [TILES] weights written to tensor memory
+  const uint32_t bar_o = bar_p + 8 * TILES;          // [TILES] result complete
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 512);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + 516);
+  volatile int *unclean = reinterpret_cast<volatile int *>(tail + 520);   // non-finite values where the mask hides some of them
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   const int kh = blockIdx.x % p.kv_heads;
-  const PromptTile t = find_tile<PU_THREADS>(p, blockIdx.x / p.kv_heads);
+  const PromptTile t = find_tile<Cfg::THREADS>(p, blockIdx.x / p.kv_heads);
   if (t.queries == 0) return;
+  const int per = 128 / p.group;                                           // queries of a tile of rows
   const int lim_lo = seen(p, t, 0), lim_hi = seen(p, t, t.queries - 1);   // keys that the first and the last query see
-  const int n = (lim_hi + PU_KEYS - 1) / PU_KEYS;                          // tiles of keys
+  const int n = (lim_hi + KEYS - 1) / KEYS;                                // tiles of keys; they are taken from the last to the first
+  // a tile of rows whose last query sees fewer keys starts later; one without queries has no turn
+  auto first_turn = [&](int x) {
+    const int have = min(per, t.queries - x * per);
+    return have <= 0 ? n : n - (seen(p, t, x * per + have - 1) + KEYS - 1) / KEYS;
+  };
 
   if (tid == 0) {
     mbar_init(bar_q, 1);
     for (int s = 0; s < ST; ++s) {
-      mbar_init(bar_kf + 8 * s, 1);
-      mbar_init(bar_ke + 8 * s, 1);
-      mbar_init(bar_vf + 8 * s, 1);
-      mbar_init(bar_ve + 8 * s, 1);
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
     }
-    mbar_init(bar_s, 1);
-    mbar_init(bar_se, 4);
-    mbar_init(bar_p, 4);
-    mbar_init(bar_o, 1);
+    for (int x = 0; x < TILES; ++x) {
+      mbar_init(bar_s + 8 * x, 1);
+      mbar_init(bar_se + 8 * x, 4);
+      mbar_init(bar_p + 8 * x, 4);
+      mbar_init(bar_o + 8 * x, 2);   // the product, and the issuer's word on `unclean`
+    }
     *abort_flag = 0;
     *unclean = 0;
     fence_barrier_init();
   }
-  if (warp == 5) {
+  if (warp == 4 * TILES + 1) {
     tmem_alloc(smem_u32(tmem_slot), Cfg::COLS);
     tmem_relinquish();
   }
@@ -282,21 +310,21 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 4) {
+  if (warp == 4 * TILES) {
     if (lane == 0 && n > 0) {
       bool ok = true;
-      mbar_arrive_expect_tx(bar_q, Cfg::PANELS * 128 * p.group * p.tokens);
-      for (int c = 0; c < Cfg::PANELS; ++c) tma_load_3d(sm_q + c * 16384, &tm_q, bar_q, 64 * c, kh * p.group, t.q0);
-      for (int it = 0; it < n && ok; ++it) {
-        const uint32_t st = it % ST, ph = (it / ST) & 1;
-        const int row = t.k0 + (n - 1 - it) * PU_KEYS;
-        const uint32_t dk = sm_kv + st * 2 * Cfg::TILE, dv = dk + Cfg::TILE;
-        if (!(ok = mbar_wait(bar_ke + 8 * st, ph ^ 1u, abort_flag))) break;
-        mbar_arrive_expect_tx(bar_kf + 8 * st, Cfg::TILE);
-        for (int c = 0; c < Cfg::PANELS; ++c) tma_load_3d(dk + c * 16384, &tm_k, bar_kf + 8 * st, 64 * c, kh, row);
-        if (!(ok = mbar_wait(bar_ve + 8 * st, ph ^ 1u, abort_flag))) break;
-        mbar_arrive_expect_tx(bar_vf + 8 * st, Cfg::TILE);
-        for (int c = 0; c < Cfg::PANELS; ++c) tma_load_3d(dv + c * 16384, &tm_v, bar_vf + 8 * st, 64 * c, kh, row);
+      const int tiles = first_turn(TILES - 1) < n ? TILES : 1;
+      mbar_arrive_expect_tx(bar_q, tiles * Cfg::PANELS * 128 * p.group * per);
+      for (int x = 0; x < tiles; ++x)
+        for (int c = 0; c < Cfg::PANELS; ++c)
+          tma_load_3d(sm_q + (x * Cfg::PANELS + c) * 16384, &tm_q, bar_q, 64 * c, kh * p.group, t.q0 + x * per);
+      for (int i = 0; i < 2 * n; ++i) {   // K and V in turn
+        const uint32_t st = i % ST, ph = (i / ST) & 1;
+        const int row = t.k0 + (n - 1 - (i >> 1)) * KEYS;
+        if (!(ok = mbar_wait_relaxed(bar_empty + 8 * st, ph ^ 1u, abort_flag))) break;
+        mbar_arrive_expect_tx(bar_full + 8 * st, Cfg::TILE);
+        for (int c = 0; c < Cfg::PANELS; ++c)
+          tma_load_3d(sm_ring + st * Cfg::TILE + c * Cfg::PANEL, i & 1 ? &tm_v : &tm_k, bar_full + 8 * st, 64 * c, kh, row);
       }
       if (!ok) {
         *abort_flag = 1;
@@ -305,125 +333,188 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         while (globaltimer() - t0 < 200000ull) {}
       }
     }
-  } else if (warp == 5) {
-    if (lane == 0 && n > 0) {
-      // descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, version 1
-      const uint64_t desc_hi = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;
-      const uint32_t kmajor = 1u << 16, mnmajor = (16384u >> 4) << 16;   // MN-major: leading offset = one panel
-      const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-      const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
-      bool ok = true;
-      auto scores = [&](int it) -> bool {
-        const uint32_t st = it % ST, ph = (it / ST) & 1;
-        if (!mbar_wait(bar_kf + 8 * st, ph, abort_flag)) return false;
+  } else if (warp == 4 * TILES + 1) {
+    // descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, version 1
+    const uint64_t desc_hi = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;
+    const uint32_t kmajor = 1u << 16, mnmajor = ((uint32_t)Cfg::PANEL >> 4) << 16;   // MN-major: leading offset = one panel
+    const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | (((uint32_t)KEYS >> 3) << 17) | ((128u >> 4) << 24);
+    const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
+    int begin[TILES];
+    for (int x = 0; x < TILES; ++x) begin[x] = first_turn(x);
+    bool ok = true;
+    auto scores = [&](int x, int it) -> bool {
+      const uint32_t st = (2 * it) % ST, ph = ((2 * it) / ST) & 1;
+      if (it >= begin[x]) {
+        if (!warp_wait(bar_full + 8 * st, ph, abort_flag)) return false;
         tc_fence_after();
-        const uint32_t k = sm_kv + st * 2 * Cfg::TILE;
+        if (lane == 0) {
+          const uint32_t q = sm_q + x * Cfg::PANELS * 16384, k = sm_ring + st * Cfg::TILE;
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-          umma<KIND_F16>(tmem, desc_hi | (uint64_t)(kmajor | (((sm_q + off) >> 4) & 0x3fffu)), desc_hi | (uint64_t)(kmajor | (((k + off) >> 4) & 0x3fffu)),
-                         idesc_s, kk != 0);
+          for (int kk = 0; kk < DP / 16; ++kk)
+            umma<KIND_F16>(tmem + Cfg::S_COL + x * Cfg::STEP,
+                           desc_hi | (uint64_t)(kmajor | (((q + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4) & 0x3fffu)),
+                           desc_hi | (uint64_t)(kmajor | (((k + (kk >> 2) * Cfg::PANEL + (kk & 3) * 32) >> 4) & 0x3fffu)), idesc_s, kk != 0);
+          tc_commit(bar_s + 8 * x);
         }
-        tc_commit(bar_s);
-        tc_commit(bar_ke + 8 * st);
-        return true;
-      };
-      ok = mbar_wait(bar_q, 0, abort_flag) && scores(0);
-      for (int it = 0; it < n && ok; ++it) {
-        const uint32_t st = it % ST, ph = (it / ST) & 1;
-        if (Cfg::EARLY && it + 1 < n && !(ok = mbar_wait(bar_se, it & 1, abort_flag) && scores(it + 1))) break;
-        if (!(ok = mbar_wait(bar_p, it & 1, abort_flag) && mbar_wait(bar_vf + 8 * st, ph, abort_flag))) break;
-        tc_fence_after();
-        const uint32_t v = sm_kv + st * 2 * Cfg::TILE + Cfg::TILE;
-#pragma unroll
-        for (int kk = 0; kk < PU_KEYS / 16; ++kk)   // 16 keys: 8 columns of P, 16 rows of V
-          umma_ts(tmem + Cfg::O_COL, tmem + Cfg::P_COL + 8 * kk, desc_hi | (uint64_t)(mnmajor | (((v + 2048 * kk) >> 4) & 0x3fffu)), idesc_o,
-                  it != 0 || kk != 0);
-        tc_commit(bar_ve + 8 * st);
-        if (it + 1 == n) tc_commit(bar_o);
-        // without columns of their own the weights lie where the next scores go: that product follows this one in the pipe
-        if (!Cfg::EARLY && it + 1 < n && !(ok = scores(it + 1))) break;
       }
-      if (!ok) {
-        *abort_flag = 1;
-        report(p.status, DEV_WAIT_SMEM_FULL);
+      if (x == TILES - 1 && lane == 0) tc_commit(bar_empty + 8 * st);   // both tiles' products with these keys are on their way
+      return true;
+    };
+    if (n > 0) ok = warp_wait(bar_q, 0, abort_flag);
+    for (int x = 0; x < TILES && n > 0 && ok; ++x) ok = scores(x, 0);
+    for (int it = 0; it < n && ok; ++it) {
+      const int base = (n - 1 - it) * KEYS;
+      const uint32_t st = (2 * it + 1) % ST, ph = ((2 * it + 1) / ST) & 1;
+      if (Cfg::EARLY && it + 1 < n && !(ok = warp_wait(bar_se, it & 1, abort_flag) && scores(0, it + 1))) break;
+      if (!(ok = warp_wait(bar_full + 8 * st, ph, abort_flag))) break;
+      if (base + KEYS > lim_lo) {
+        // Values past the last key that anybody here sees belong to others and may hold anything: zeros in their place, since
+        // the tensor cores multiply every value by every row's weight and 0 * NaN is NaN.  Values on the diagonal are hidden
+        // from some rows only: if one is not finite, the rows are summed up the plain way at the end.
+        uint8_t *v = gen + Cfg::Q + st * Cfg::TILE;
+        constexpr int PIECES = 8 * Cfg::PANELS;   // 16-byte pieces of a key's values
+        const int none = max(0, min(KEYS, lim_hi - base)), some = max(0, min(none, lim_lo - base));
+        for (int i = none * PIECES + lane; i < KEYS * PIECES; i += 32) {
+          const int key = i / PIECES, piece = i % PIECES;
+          *reinterpret_cast<uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        bool bad = false;
+        for (int i = some * PIECES + lane; i < none * PIECES; i += 32) {
+          const int key = i / PIECES, piece = i % PIECES;
+          const uint4 w = *reinterpret_cast<const uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16);
+          for (uint32_t u : {w.x, w.y, w.z, w.w}) bad |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
+        }
+        if (bad) *unclean = 1;
+        fence_proxy_async();
+        __syncwarp();
+      }
+      for (int x = 0; x < TILES; ++x) {
+        if (it >= begin[x]) {
+          if (!(ok = warp_wait(bar_p + 8 * x, (it - begin[x]) & 1, abort_flag))) break;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t v = sm_ring + st * Cfg::TILE;
+#pragma unroll
+            for (int kk = 0; kk < KEYS / 16; ++kk)   // 16 keys: 8 columns of P, 16 rows of V
+              umma_ts(tmem + Cfg::O_COL + x * Cfg::STEP, tmem + Cfg::P_COL + x * Cfg::STEP + 8 * kk,
+                      desc_hi | (uint64_t)(mnmajor | (((v + 2048 * kk) >> 4) & 0x3fffu)), idesc_o, it != begin[x] || kk != 0);
+          }
+        }
+        if (lane == 0) {
+          if (x == TILES - 1) tc_commit(bar_empty + 8 * st);
+          if (it + 1 == n && begin[x] < n) {
+            tc_commit(bar_o + 8 * x);
+            mbar_arrive(bar_o + 8 * x);
+          }
+        }
+        // Without columns of their own the weights lie where the next scores go.  Both products are this thread's, and the
+        // tensor cores take them in order.
+        if (!Cfg::EARLY && it + 1 < n && !(ok = scores(x, it + 1))) break;
       }
     }
+    if (!ok && lane == 0) {
+      *abort_flag = 1;
+      report(p.status, DEV_WAIT_SMEM_FULL);
+    }
   } else {
-    const int row = warp * 32 + lane;
-    const int query = row / p.group, head = row - query * p.group;
-    const bool mine = query < t.queries;          // rows past the tile's last query (and past tokens * group) hold anything
+    const int x = warp >> 2;                      // tile of rows
+    const int row = (warp & 3) * 32 + lane;
+    const int in_tile = row / p.group, head = row - in_tile * p.group, query = x * per + in_tile;
+    const bool mine = in_tile < per && query < t.queries;   // rows past the last query (and past per * group) hold anything
     const int lim = mine ? seen(p, t, query) : lim_hi;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const uint32_t t_s = tmem + lanes, t_p = t_s + Cfg::P_COL, t_o = t_s + Cfg::O_COL;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + Cfg::S_COL + x * Cfg::STEP, t_p = tmem + lanes + Cfg::P_COL + x * Cfg::STEP;
+    const uint32_t t_o = tmem + lanes + Cfg::O_COL + x * Cfg::STEP;
     const float c = p.scale_log2e;
     float m = -INFINITY, l = 0.f;   // reference maximum of the unscaled scores; sum of the weights
+    const int begin = first_turn(x);
     bool ok = true;
-    for (int it = 0; it < n; ++it) {
-      const int base = (n - 1 - it) * PU_KEYS;
-      const uint32_t st = it % ST, ph = (it / ST) & 1;
-      if (!(ok = mbar_wait(bar_s, it & 1, abort_flag))) break;
+    for (int it = begin; it < n; ++it) {
+      const int base = (n - 1 - it) * KEYS, turn = it - begin;
+      if (!(ok = warp_wait(bar_s + 8 * x, turn & 1, abort_flag))) break;
       tc_fence_after();
-      uint32_t r[PU_KEYS];
-      float *s = reinterpret_cast<float *>(r);
-      tmem_ld_x32(t_s, r);
-      tmem_ld_x32(t_s + 32, r + 32);
-      tmem_ld_x32(t_s + 64, r + 64);
-      tmem_ld_x32(t_s + 96, r + 96);
-      tmem_ld_wait();
-      if (Cfg::EARLY) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_se);
-      }
-      const bool masked = base + PU_KEYS > lim_lo;
-      if (masked) {
-        const int have = lim - base;
+      const int have = base + KEYS > lim_lo ? lim - base : KEYS;   // keys of this tile that the row sees
+      const bool masked = base + KEYS > lim_lo;
+      constexpr int HELD = Cfg::HOLD ? KEYS : 32;
+      uint32_t r[HELD];
+      float top = -INFINITY;
+      auto take = [&](uint32_t *w, int at) {   // 32 scores: masks, maximum
+        float *s = reinterpret_cast<float *>(w);
+        if (masked)
 #pragma unroll
-        for (int i = 0; i < PU_KEYS; ++i) s[i] = i < have ? s[i] : -INFINITY;
-      }
-      float x0 = s[0], x1 = s[1], x2 = s[2], x3 = s[3];
+          for (int i = 0; i < 32; ++i) s[i] = at + i < have ? s[i] : -INFINITY;
+        float x0 = s[0], x1 = s[1];
 #pragma unroll
-      for (int i = 4; i < PU_KEYS; i += 4) {
-        x0 = fmaxf(x0, s[i]);
-        x1 = fmaxf(x1, s[i + 1]);
-        x2 = fmaxf(x2, s[i + 2]);
-        x3 = fmaxf(x3, s[i + 3]);
+        for (int i = 2; i < 32; i += 2) {
+          x0 = fmaxf(x0, s[i]);
+          x1 = fmaxf(x1, s[i + 1]);
+        }
+        top = fmaxf(top, fmaxf(x0, x1));
+      };
+      if constexpr (Cfg::HOLD) {
+#pragma unroll
+        for (int i = 0; i < KEYS; i += 32) tmem_ld_x32(t_s + i, r + i);
+        tmem_ld_wait();
+        if (Cfg::EARLY) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_se + 8 * x);
+        }
+#pragma unroll
+        for (int i = 0; i < KEYS; i += 32) take(r + i, i);
+      } else {
+        uint32_t other[32];
+#pragma unroll
+        for (int i = 0; i < KEYS; i += 64) {
+          if (i == 0) tmem_ld_x32(t_s, r);
+          tmem_ld_wait();
+          tmem_ld_x32(t_s + i + 32, other);
+          take(r, i);
+          tmem_ld_wait();
+          tmem_ld_x32(t_s + (i + 64) % KEYS, r);   // at the end the first 32 once more
+          take(other, i + 32);
+        }
       }
-      const float top = fmaxf(fmaxf(x0, x1), fmaxf(x2, x3));
-      if (Cfg::EARLY && it > 0) {   // O and P are free
-        if (!(ok = mbar_wait(bar_ve + 8 * ((it - 1) % ST), ((it - 1) / ST) & 1, abort_flag))) break;
+      if (Cfg::EARLY && turn > 0) {   // the previous product has left P and O
+        const int i = 2 * it - 1;
+        if (!(ok = warp_wait(bar_empty + 8 * (i % ST), (i / ST) & 1, abort_flag))) break;
         tc_fence_after();
       }
-      if (it == 0) {
+      if (turn == 0) {
         m = top;
       } else {
         const bool up = (top - m) * c > 8.f;
         if (__any_sync(0xffffffffu, up)) {
-          tc_fence_after();
           const float f = up ? ex2((m - top) * c) : 1.f;
           if (up) m = top;
           l *= f;
+          if constexpr (!Cfg::HOLD) tmem_ld_wait();
 #pragma unroll
-          for (int d = 0; d < DP; d += 32) {
-            uint32_t o[32];
-            tmem_ld_x32(t_o + d, o);
+          for (int d = 0; d < DP; d += 16) {
+            uint32_t o[16];
+            tmem_ld_x16(t_o + d, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st_x32(t_o + d, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st_x16(t_o + d, o);
           }
         }
       }
       const float off = m == -INFINITY ? 0.f : -m * c;
       const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
       float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+      auto weigh = [&](const uint32_t *from, int at) {   // 32 scores -> 16 columns of P
+        const float *s = reinterpret_cast<const float *>(from);
+        uint32_t w[16];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float2 e = __ffma2_rn(make_float2(s[half * 64 + 2 * i], s[half * 64 + 2 * i + 1]), c2, off2);
+        for (int i = 0; i < 16; ++i) {
+          float2 e = make_float2(s[2 * i], s[2 * i + 1]);
+          if constexpr (!Cfg::HOLD)
+            if (masked) {
+              e.x = at + 2 * i < have ? e.x : -INFINITY;
+              e.y = at + 2 * i + 1 < have ? e.y : -INFINITY;
+            }
+          e = __ffma2_rn(e, c2, off2);
           e.x = ex2(e.x);
           e.y = ex2(e.y);
           if (i & 1) sum1 = __fadd2_rn(sum1, e);
@@ -431,38 +522,37 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
           w[i] = *reinterpret_cast<const uint32_t *>(&h);
         }
-        tmem_st_x32(t_p + 32 * half, w);
+        tmem_st_x16(t_p + at / 2, w);
+      };
+      if constexpr (Cfg::HOLD) {
+#pragma unroll
+        for (int i = 0; i < KEYS; i += 32) weigh(r + i, i);
+      } else {
+        uint32_t other[32];
+#pragma unroll
+        for (int i = 0; i < KEYS; i += 64) {
+          tmem_ld_wait();
+          tmem_ld_x32(t_s + i + 32, other);
+          weigh(r, i);
+          tmem_ld_wait();
+          if (i + 64 < KEYS) tmem_ld_x32(t_s + i + 64, r);
+          weigh(other, i + 32);
+        }
       }
       l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-      if (masked) {
-        // Values past the tile's last key belong to others and may hold anything: zeros in their place.  Values on the diagonal
-        // are hidden from some rows: if one is not finite, the rows are computed the plain way at the end.
-        if (!(ok = mbar_wait(bar_vf + 8 * st, ph, abort_flag))) break;
-        uint8_t *v = gen + (sm_kv - sm_q) + st * 2 * Cfg::TILE + Cfg::TILE;
-        const int none = max(0, min(PU_KEYS, lim_hi - base)), some = max(0, min(none, lim_lo - base));
-        for (int i = none * 8 * Cfg::PANELS + tid; i < PU_KEYS * 8 * Cfg::PANELS; i += 128) {
-          const int key = i / (8 * Cfg::PANELS), piece = i % (8 * Cfg::PANELS);
-          *reinterpret_cast<uint4 *>(v + (piece >> 3) * 16384 + key * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        bool bad = false;
-        for (int i = some * 8 * Cfg::PANELS + tid; i < none * 8 * Cfg::PANELS; i += 128) {
-          const int key = i / (8 * Cfg::PANELS), piece = i % (8 * Cfg::PANELS);
-          const uint4 x = *reinterpret_cast<const uint4 *>(v + (piece >> 3) * 16384 + key * 128 + (piece & 7) * 16);
-          for (uint32_t u : {x.x, x.y, x.z, x.w}) bad |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
-        }
-        if (bad) *unclean = 1;
-        fence_proxy_async();
-      }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_p);
+      if (lane == 0) {
+        if (Cfg::EARLY && !Cfg::HOLD) mbar_arrive(bar_se + 8 * x);
+        mbar_arrive(bar_p + 8 * x);
+      }
     }
-    if (ok && n > 0) ok = mbar_wait(bar_o, 0, abort_flag);
+    if (ok && begin < n) ok = warp_wait(bar_o + 8 * x, 0, abort_flag);
     if (!ok) {
       *abort_flag = 1;
       report(p.status, DEV_WAIT_TMEM_FULL);
-    } else {
+    } else if (x * per < t.queries) {
       tc_fence_after();
       const long long q_row = (long long)t.q0 + query;
       if (n > 0 && *unclean) {
@@ -470,13 +560,13 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       } else {
         // through shared memory (the queries are read), so that a row leaves in whole lines
         const float inv = 1.f / l;
-        const bool none = lim <= 0;
+        const bool none = begin == n || lim <= 0;
         constexpr int PIECES = DP / 8;
-        uint8_t *out = gen + warp * 32 * (DP * 2);
+        uint8_t *out = gen + x * Cfg::PANELS * 16384 + (warp & 3) * 32 * (DP * 2);
 #pragma unroll
         for (int d = 0; d < DP; d += 32) {
           uint32_t o[32];
-          if (n > 0) {
+          if (begin < n) {
             tmem_ld_x32(t_o + d, o);
             tmem_ld_wait();
           }
@@ -485,8 +575,8 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             uint32_t w[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const __nv_bfloat162 h = n > 0 && !none ? __floats2bfloat162_rn(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv)
-                                                      : __floats2bfloat162_rn(0.f, 0.f);
+              const __nv_bfloat162 h = none ? __floats2bfloat162_rn(0.f, 0.f)
+                                            : __floats2bfloat162_rn(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
               w[k] = *reinterpret_cast<const uint32_t *>(&h);
             }
             const int piece = (d + i) / 8;
@@ -497,10 +587,10 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         __nv_bfloat16 *y = static_cast<__nv_bfloat16 *>(p.y) + (long long)t.q0 * p.ldy + (long long)kh * p.group * p.dim;
 #pragma unroll 4
         for (int i = lane; i < 32 * PIECES; i += 32) {
-          const int r = i / PIECES, piece = i % PIECES, at = warp * 32 + r;
-          const int qi = at / p.group, hi = at - qi * p.group;
-          if (qi < t.queries && piece * 8 < p.dim)
-            *reinterpret_cast<uint4 *>(y + qi * p.ldy + hi * p.dim + piece * 8) = *reinterpret_cast<const uint4 *>(out + r * (DP * 2) + ((piece ^ (r & 7)) << 4));
+          const int rr = i / PIECES, piece = i % PIECES, at = (warp & 3) * 32 + rr;
+          const int qi = at / p.group, hi = at - qi * p.group, qq = x * per + qi;
+          if (qi < per && qq < t.queries && piece * 8 < p.dim)
+            *reinterpret_cast<uint4 *>(y + qq * p.ldy + hi * p.dim + piece * 8) = *reinterpret_cast<const uint4 *>(out + rr * (DP * 2) + ((piece ^ (rr & 7)) << 4));
         }
       }
     }
@@ -508,7 +598,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 4 * TILES + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, Cfg::COLS);
   }
@@ -541,16 +631,21 @@ static int encode_rows(CUtensorMap *tm, const void *base, int dim, int heads, lo
 }
 
 template <int DP>
-static int launch_umma(sofie_b200_ctx *ctx, const PromptParams &p, unsigned grid) {
+static int launch_umma(sofie_b200_ctx *ctx, PromptParams p) {
+  using Cfg = UmmaSize<DP>;
+  const int per = 128 / p.group;
+  p.tokens = Cfg::TILES * per;
+  const long long grid = (p.q_rows / p.tokens + p.batch) * p.kv_heads;   // every sequence may end inside a tile
+  if (grid > 0x7fffffffLL) return fail(SOFIE_B200_ERR_TOO_LARGE, "prompt_attention_enqueue: %lld queries of %d heads", p.q_rows, p.heads);
   CUtensorMap tm_q, tm_k, tm_v;
   const void *k = p.k_rows ? p.k : p.q, *v = p.k_rows ? p.v : p.q;   // no keys: nothing is loaded, but a map has to describe something
   const long long k_rows = p.k_rows ? p.k_rows : 1;
   int rc;
-  if ((rc = encode_rows(&tm_q, p.q, p.dim, p.heads, p.q_rows, p.ldq, p.group, p.tokens))) return rc;
-  if ((rc = encode_rows(&tm_k, k, p.dim, p.kv_heads, k_rows, p.ldk, 1, PU_KEYS))) return rc;
-  if ((rc = encode_rows(&tm_v, v, p.dim, p.kv_heads, k_rows, p.ldv, 1, PU_KEYS))) return rc;
-  SB_CUDA(cudaFuncSetAttribute(prompt_umma_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, UmmaCfg<DP>::SMEM));   // per device
-  prompt_umma_kernel<DP><<<grid, PU_THREADS, UmmaCfg<DP>::SMEM, ctx->stream>>>(tm_q, tm_k, tm_v, p);
+  if ((rc = encode_rows(&tm_q, p.q, p.dim, p.heads, p.q_rows, p.ldq, p.group, per))) return rc;
+  if ((rc = encode_rows(&tm_k, k, p.dim, p.kv_heads, k_rows, p.ldk, 1, Cfg::KEYS))) return rc;
+  if ((rc = encode_rows(&tm_v, v, p.dim, p.kv_heads, k_rows, p.ldv, 1, Cfg::KEYS))) return rc;
+  SB_CUDA(cudaFuncSetAttribute(prompt_umma_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));   // per device
+  prompt_umma_kernel<DP><<<(unsigned)grid, Cfg::THREADS, Cfg::SMEM, ctx->stream>>>(tm_q, tm_k, tm_v, p);
   SB_CUDA(cudaGetLastError());
   ctx->launches++;
   return 0;
@@ -628,12 +723,9 @@ int sofie_b200_prompt_attention_enqueue(sofie_b200_prompt_attention_plan *plan, 
   p.scale_log2e = d.scale * 1.4426950408889634f;
   p.status = ctx->d_status;
   if (d.dtype == SOFIE_B200_BF16) {
-    p.tokens = 128 / p.group;
-    const int64_t blocks = (q_tokens / p.tokens + batch) * d.kv_heads;   // every sequence may end inside a tile
-    if (blocks > 0x7fffffffLL) return fail(SOFIE_B200_ERR_TOO_LARGE, "prompt_attention_enqueue: %lld queries of %d heads", (long long)q_tokens, d.heads);
-    if (d.head_dim <= 64) return launch_umma<64>(ctx, p, (unsigned)blocks);
-    if (d.head_dim <= 128) return launch_umma<128>(ctx, p, (unsigned)blocks);
-    return launch_umma<256>(ctx, p, (unsigned)blocks);
+    if (d.head_dim <= 64) return launch_umma<64>(ctx, p);
+    if (d.head_dim <= 128) return launch_umma<128>(ctx, p);
+    return launch_umma<256>(ctx, p);
   }
   const int64_t blocks = (q_tokens * d.heads + 3) / 4;
   if (blocks > 0x7fffffffLL) return fail(SOFIE_B200_ERR_TOO_LARGE, "prompt_attention_enqueue: %lld queries of %d heads", (long long)q_tokens, d.heads);
