@@ -9,6 +9,7 @@
 #include <math.h>
 #include <mutex>
 #include <new>
+#include <type_traits>
 
 #include "generate.cuh"
 #include "ptx.cuh"
@@ -160,14 +161,60 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// D (tensor memory) += A (tensor memory: 128 rows, two bf16 per 32-bit column) * B (shared memory)
-__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// max(a, b, c), NaN if one of them is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// 2^x for x <= 2^7 on the FMA pipes: the special-function unit does 16 exponentials a cycle and SM, as long for a tile's scores as the
+// tensor cores need for both products, so some of them go another way.  x = n + r with n the nearest integer (x + 1.5 * 2^23
+// leaves n in the low bits), 2^r on [-1/2, 1/2] by the polynomial of degree 4 with p(0) = 1 whose largest relative error is
+// least (2.9e-6, fitted to 2^r by linear programming), n added to the exponent.  Below -127 the result is 0, as ex2 flushes.
+__device__ __forceinline__ float2 exp2_pair(float2 x) {
+  x.x = fmaxf(x.x, -127.f);
+  x.y = fmaxf(x.y, -127.f);
+  const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));
+  const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+  const float2 r = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+  float2 p = __ffma2_rn(r, make_float2(0.0095828529f, 0.0095828529f), make_float2(0.0559064262f, 0.0559064262f));
+  p = __ffma2_rn(p, r, make_float2(0.2402409911f, 0.2402409911f));
+  p = __ffma2_rn(p, r, make_float2(0.6931241751f, 0.6931241751f));
+  p = __ffma2_rn(p, r, make_float2(1.f, 1.f));
+  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
+}
+#ifndef SB_POLY
+#define SB_POLY 0x8888u
+#endif
+constexpr uint32_t POLY = SB_POLY;   // of 16 pairs, those that exp2_pair takes
+// The issuing warp stays together and one lane's predicate does the rest: the operands are then the same in every lane, which
+// lets the compiler keep them in uniform registers.  With a branch to one lane around the products every operand was moved there
+// one by one, and issuing a tile's 16 products took longer than computing them.
+// D (tensor memory) = or += A (shared memory) * B (shared memory)
+__device__ __forceinline__ void umma_ss(uint32_t leader, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
+// the same with A in tensor memory (128 rows, two bf16 per 32-bit column)
+__device__ __forceinline__ void umma_ts(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.b32 p, %4, 0;\nsetp.ne.b32 q, %5, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit_if(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred q;\nsetp.ne.b32 q, %1, 0;\n"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
+      "r"(leader)
+      : "memory");
+}
+// A value that all lanes hold, as one.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
 __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t *r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
@@ -210,7 +257,10 @@ struct UmmaSize : UmmaCfg<DP> {
   static constexpr int Q = C::TILES * PANELS * 16384;
   static constexpr int TILE = C::KEYS * DP * 2;             // keys or values
   static constexpr int PANEL = C::KEYS * 128;
-  static constexpr int THREADS = C::TILES * 128 + 64;       // warps of rows; then TMA, MMA
+  // Warps of rows; then TMA, MMA.  Where a thread holds a row of 128 scores, 168 registers (12 warps' share) make it spill: the block
+  // is launched with a whole third group of warps, which hands registers over, 384 x 168 = 256 x 216 + 128 x 72.
+  static constexpr bool MOVE = C::TILES == 2;
+  static constexpr int THREADS = C::TILES * 128 + (MOVE ? 128 : 64);
   static constexpr int SMEM = Q + C::STAGES * TILE + 1024 /*barriers*/ + 1024 /*alignment*/;
 };
 
@@ -310,113 +360,8 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 4 * TILES) {
-    if (lane == 0 && n > 0) {
-      bool ok = true;
-      const int tiles = first_turn(TILES - 1) < n ? TILES : 1;
-      mbar_arrive_expect_tx(bar_q, tiles * Cfg::PANELS * 128 * p.group * per);
-      for (int x = 0; x < tiles; ++x)
-        for (int c = 0; c < Cfg::PANELS; ++c)
-          tma_load_3d(sm_q + (x * Cfg::PANELS + c) * 16384, &tm_q, bar_q, 64 * c, kh * p.group, t.q0 + x * per);
-      for (int i = 0; i < 2 * n; ++i) {   // K and V in turn
-        const uint32_t st = i % ST, ph = (i / ST) & 1;
-        const int row = t.k0 + (n - 1 - (i >> 1)) * KEYS;
-        if (!(ok = mbar_wait_relaxed(bar_empty + 8 * st, ph ^ 1u, abort_flag))) break;
-        mbar_arrive_expect_tx(bar_full + 8 * st, Cfg::TILE);
-        for (int c = 0; c < Cfg::PANELS; ++c)
-          tma_load_3d(sm_ring + st * Cfg::TILE + c * Cfg::PANEL, i & 1 ? &tm_v : &tm_k, bar_full + 8 * st, 64 * c, kh, row);
-      }
-      if (!ok) {
-        *abort_flag = 1;
-        report(p.status, DEV_WAIT_SMEM_EMPTY);
-        const uint64_t t0 = globaltimer();   // copies in flight land before the block ends
-        while (globaltimer() - t0 < 200000ull) {}
-      }
-    }
-  } else if (warp == 4 * TILES + 1) {
-    // descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, version 1
-    const uint64_t desc_hi = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;
-    const uint32_t kmajor = 1u << 16, mnmajor = ((uint32_t)Cfg::PANEL >> 4) << 16;   // MN-major: leading offset = one panel
-    const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | (((uint32_t)KEYS >> 3) << 17) | ((128u >> 4) << 24);
-    const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
-    int begin[TILES];
-    for (int x = 0; x < TILES; ++x) begin[x] = first_turn(x);
-    bool ok = true;
-    auto scores = [&](int x, int it) -> bool {
-      const uint32_t st = (2 * it) % ST, ph = ((2 * it) / ST) & 1;
-      if (it >= begin[x]) {
-        if (!warp_wait(bar_full + 8 * st, ph, abort_flag)) return false;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t q = sm_q + x * Cfg::PANELS * 16384, k = sm_ring + st * Cfg::TILE;
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk)
-            umma<KIND_F16>(tmem + Cfg::S_COL + x * Cfg::STEP,
-                           desc_hi | (uint64_t)(kmajor | (((q + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4) & 0x3fffu)),
-                           desc_hi | (uint64_t)(kmajor | (((k + (kk >> 2) * Cfg::PANEL + (kk & 3) * 32) >> 4) & 0x3fffu)), idesc_s, kk != 0);
-          tc_commit(bar_s + 8 * x);
-        }
-      }
-      if (x == TILES - 1 && lane == 0) tc_commit(bar_empty + 8 * st);   // both tiles' products with these keys are on their way
-      return true;
-    };
-    if (n > 0) ok = warp_wait(bar_q, 0, abort_flag);
-    for (int x = 0; x < TILES && n > 0 && ok; ++x) ok = scores(x, 0);
-    for (int it = 0; it < n && ok; ++it) {
-      const int base = (n - 1 - it) * KEYS;
-      const uint32_t st = (2 * it + 1) % ST, ph = ((2 * it + 1) / ST) & 1;
-      if (Cfg::EARLY && it + 1 < n && !(ok = warp_wait(bar_se, it & 1, abort_flag) && scores(0, it + 1))) break;
-      if (!(ok = warp_wait(bar_full + 8 * st, ph, abort_flag))) break;
-      if (base + KEYS > lim_lo) {
-        // Values past the last key that anybody here sees belong to others and may hold anything: zeros in their place, since
-        // the tensor cores multiply every value by every row's weight and 0 * NaN is NaN.  Values on the diagonal are hidden
-        // from some rows only: if one is not finite, the rows are summed up the plain way at the end.
-        uint8_t *v = gen + Cfg::Q + st * Cfg::TILE;
-        constexpr int PIECES = 8 * Cfg::PANELS;   // 16-byte pieces of a key's values
-        const int none = max(0, min(KEYS, lim_hi - base)), some = max(0, min(none, lim_lo - base));
-        for (int i = none * PIECES + lane; i < KEYS * PIECES; i += 32) {
-          const int key = i / PIECES, piece = i % PIECES;
-          *reinterpret_cast<uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        bool bad = false;
-        for (int i = some * PIECES + lane; i < none * PIECES; i += 32) {
-          const int key = i / PIECES, piece = i % PIECES;
-          const uint4 w = *reinterpret_cast<const uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16);
-          for (uint32_t u : {w.x, w.y, w.z, w.w}) bad |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
-        }
-        if (bad) *unclean = 1;
-        fence_proxy_async();
-        __syncwarp();
-      }
-      for (int x = 0; x < TILES; ++x) {
-        if (it >= begin[x]) {
-          if (!(ok = warp_wait(bar_p + 8 * x, (it - begin[x]) & 1, abort_flag))) break;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t v = sm_ring + st * Cfg::TILE;
-#pragma unroll
-            for (int kk = 0; kk < KEYS / 16; ++kk)   // 16 keys: 8 columns of P, 16 rows of V
-              umma_ts(tmem + Cfg::O_COL + x * Cfg::STEP, tmem + Cfg::P_COL + x * Cfg::STEP + 8 * kk,
-                      desc_hi | (uint64_t)(mnmajor | (((v + 2048 * kk) >> 4) & 0x3fffu)), idesc_o, it != begin[x] || kk != 0);
-          }
-        }
-        if (lane == 0) {
-          if (x == TILES - 1) tc_commit(bar_empty + 8 * st);
-          if (it + 1 == n && begin[x] < n) {
-            tc_commit(bar_o + 8 * x);
-            mbar_arrive(bar_o + 8 * x);
-          }
-        }
-        // Without columns of their own the weights lie where the next scores go.  Both products are this thread's, and the
-        // tensor cores take them in order.
-        if (!Cfg::EARLY && it + 1 < n && !(ok = scores(x, it + 1))) break;
-      }
-    }
-    if (!ok && lane == 0) {
-      *abort_flag = 1;
-      report(p.status, DEV_WAIT_SMEM_FULL);
-    }
-  } else {
+  if (warp < 4 * TILES) {
+    if constexpr (Cfg::MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int x = warp >> 2;                      // tile of rows
     const int row = (warp & 3) * 32 + lane;
     const int in_tile = row / p.group, head = row - in_tile * p.group, query = x * per + in_tile;
@@ -428,30 +373,39 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const float c = p.scale_log2e;
     float m = -INFINITY, l = 0.f;   // reference maximum of the unscaled scores; sum of the weights
     const int begin = first_turn(x);
+    // a tile's maximum: moves the reference maximum if it has to, and with it the sum and O
+    auto raise = [&](float top, int turn) {
+      if (turn == 0) {
+        m = top;
+        return;
+      }
+      const bool up = (top - m) * c > 8.f;
+      if (!__any_sync(0xffffffffu, up)) return;
+      const float f = up ? ex2((m - top) * c) : 1.f;
+      if (up) m = top;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < DP; d += 16) {
+        uint32_t o[16];
+        tmem_ld_x16(t_o + d, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tmem_st_x16(t_o + d, o);
+      }
+    };
     bool ok = true;
     for (int it = begin; it < n; ++it) {
       const int base = (n - 1 - it) * KEYS, turn = it - begin;
       if (!(ok = warp_wait(bar_s + 8 * x, turn & 1, abort_flag))) break;
       tc_fence_after();
-      const int have = base + KEYS > lim_lo ? lim - base : KEYS;   // keys of this tile that the row sees
+      const int have = lim - base;   // keys of this tile that the row sees
       const bool masked = base + KEYS > lim_lo;
-      constexpr int HELD = Cfg::HOLD ? KEYS : 32;
-      uint32_t r[HELD];
-      float top = -INFINITY;
-      auto take = [&](uint32_t *w, int at) {   // 32 scores: masks, maximum
-        float *s = reinterpret_cast<float *>(w);
-        if (masked)
-#pragma unroll
-          for (int i = 0; i < 32; ++i) s[i] = at + i < have ? s[i] : -INFINITY;
-        float x0 = s[0], x1 = s[1];
-#pragma unroll
-        for (int i = 2; i < 32; i += 2) {
-          x0 = fmaxf(x0, s[i]);
-          x1 = fmaxf(x1, s[i + 1]);
-        }
-        top = fmaxf(top, fmaxf(x0, x1));
-      };
+      const float2 c2 = make_float2(c, c);
+      bool careful = masked || turn == 0;
       if constexpr (Cfg::HOLD) {
+        uint32_t r[KEYS];
+        float *s = reinterpret_cast<float *>(r);
 #pragma unroll
         for (int i = 0; i < KEYS; i += 32) tmem_ld_x32(t_s + i, r + i);
         tmem_ld_wait();
@@ -459,11 +413,88 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_se + 8 * x);
+          if (turn > 0) {   // the previous product has left P and O
+            const int i = 2 * it - 1;
+            if (!(ok = warp_wait(bar_empty + 8 * (i % ST), (i / ST) & 1, abort_flag))) break;
+            tc_fence_after();
+          }
         }
+        // 32 scores -> 16 columns of P.  MIX: the pairs of each 16 whose exponentials are a polynomial (see exp2_pair).
+        auto weigh = [&](int at, float2 off2, float2 &sum, auto mix) {
+          constexpr uint32_t MIX = decltype(mix)::value;
+          uint32_t w[16];
+          float2 other = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < KEYS; i += 32) take(r + i, i);
+          for (int i = 0; i < 16; ++i) {
+            float2 e = __ffma2_rn(make_float2(s[at + 2 * i], s[at + 2 * i + 1]), c2, off2);
+            if ((MIX >> i) & 1) {
+              e = exp2_pair(e);
+            } else {
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+            }
+            if (i & 1) other = __fadd2_rn(other, e);
+            else sum = __fadd2_rn(sum, e);
+            const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+          }
+          sum = __fadd2_rn(sum, other);
+          tmem_st_x16(t_p + at / 2, w);
+        };
+        if (!careful) {
+          // The weights by the reference maximum that is there, without waiting for this tile's own; that one is found beside
+          // them and, if it is more than 2^8 above (or a score is NaN or +inf), the tile is done over.
+          const float off = -m * c;
+          float2 sum = make_float2(0.f, 0.f);
+          float x0 = s[0], x1 = s[1];
+#pragma unroll
+          for (int i = 0; i < KEYS; i += 32) {
+            weigh(i, make_float2(off, off), sum, std::integral_constant<uint32_t, POLY>());
+#pragma unroll
+            for (int k = i; k < i + 32; k += 4) {
+              x0 = max3_nan(x0, s[k], s[k + 1]);
+              x1 = max3_nan(x1, s[k + 2], s[k + 3]);
+            }
+          }
+          const float top = max3_nan(x0, x1, x1);
+          careful = __any_sync(0xffffffffu, mine && !((top - m) * c <= 8.f));
+          if (!careful) l += sum.x + sum.y;
+        }
+        if (careful) {
+          tmem_st_wait();   // what the first attempt wrote is written again
+          if (masked)
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) s[i] = i < have ? s[i] : -INFINITY;
+          float x0 = s[0], x1 = s[1];
+#pragma unroll
+          for (int i = 2; i < KEYS; i += 2) {
+            x0 = fmaxf(x0, s[i]);
+            x1 = fmaxf(x1, s[i + 1]);
+          }
+          raise(fmaxf(x0, x1), turn);
+          const float off = m == -INFINITY ? 0.f : -m * c;
+          float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < KEYS; i += 32) weigh(i, make_float2(off, off), sum, std::integral_constant<uint32_t, 0>());
+          l += sum.x + sum.y;
+        }
       } else {
-        uint32_t other[32];
+        // twice from tensor memory, 32 columns at a time: once for the maximum, once for the weights
+        uint32_t r[32], other[32];
+        float top = -INFINITY;
+        auto take = [&](uint32_t *w, int at) {
+          float *s = reinterpret_cast<float *>(w);
+          if (masked)
+#pragma unroll
+            for (int i = 0; i < 32; ++i) s[i] = at + i < have ? s[i] : -INFINITY;
+          float x0 = s[0], x1 = s[1];
+#pragma unroll
+          for (int i = 2; i < 32; i += 2) {
+            x0 = fmaxf(x0, s[i]);
+            x1 = fmaxf(x1, s[i + 1]);
+          }
+          top = fmaxf(top, fmaxf(x0, x1));
+        };
 #pragma unroll
         for (int i = 0; i < KEYS; i += 64) {
           if (i == 0) tmem_ld_x32(t_s, r);
@@ -471,64 +502,39 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           tmem_ld_x32(t_s + i + 32, other);
           take(r, i);
           tmem_ld_wait();
-          tmem_ld_x32(t_s + (i + 64) % KEYS, r);   // at the end the first 32 once more
+          if (i + 64 < KEYS) tmem_ld_x32(t_s + i + 64, r);
           take(other, i + 32);
         }
-      }
-      if (Cfg::EARLY && turn > 0) {   // the previous product has left P and O
-        const int i = 2 * it - 1;
-        if (!(ok = warp_wait(bar_empty + 8 * (i % ST), (i / ST) & 1, abort_flag))) break;
-        tc_fence_after();
-      }
-      if (turn == 0) {
-        m = top;
-      } else {
-        const bool up = (top - m) * c > 8.f;
-        if (__any_sync(0xffffffffu, up)) {
-          const float f = up ? ex2((m - top) * c) : 1.f;
-          if (up) m = top;
-          l *= f;
-          if constexpr (!Cfg::HOLD) tmem_ld_wait();
-#pragma unroll
-          for (int d = 0; d < DP; d += 16) {
-            uint32_t o[16];
-            tmem_ld_x16(t_o + d, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st_x16(t_o + d, o);
-          }
+        if (Cfg::EARLY && turn > 0) {
+          const int i = 2 * it - 1;
+          if (!(ok = warp_wait(bar_empty + 8 * (i % ST), (i / ST) & 1, abort_flag))) break;
+          tc_fence_after();
         }
-      }
-      const float off = m == -INFINITY ? 0.f : -m * c;
-      const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
-      float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-      auto weigh = [&](const uint32_t *from, int at) {   // 32 scores -> 16 columns of P
-        const float *s = reinterpret_cast<const float *>(from);
-        uint32_t w[16];
+        raise(top, turn);
+        tmem_ld_x32(t_s, r);
+        const float off = m == -INFINITY ? 0.f : -m * c;
+        const float2 off2 = make_float2(off, off);
+        float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+        auto weigh = [&](const uint32_t *from, int at) {
+          const float *s = reinterpret_cast<const float *>(from);
+          uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float2 e = make_float2(s[2 * i], s[2 * i + 1]);
-          if constexpr (!Cfg::HOLD)
+          for (int i = 0; i < 16; ++i) {
+            float2 e = make_float2(s[2 * i], s[2 * i + 1]);
             if (masked) {
               e.x = at + 2 * i < have ? e.x : -INFINITY;
               e.y = at + 2 * i + 1 < have ? e.y : -INFINITY;
             }
-          e = __ffma2_rn(e, c2, off2);
-          e.x = ex2(e.x);
-          e.y = ex2(e.y);
-          if (i & 1) sum1 = __fadd2_rn(sum1, e);
-          else sum0 = __fadd2_rn(sum0, e);
-          const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
-          w[i] = *reinterpret_cast<const uint32_t *>(&h);
-        }
-        tmem_st_x16(t_p + at / 2, w);
-      };
-      if constexpr (Cfg::HOLD) {
-#pragma unroll
-        for (int i = 0; i < KEYS; i += 32) weigh(r + i, i);
-      } else {
-        uint32_t other[32];
+            e = __ffma2_rn(e, c2, off2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            if (i & 1) sum1 = __fadd2_rn(sum1, e);
+            else sum0 = __fadd2_rn(sum0, e);
+            const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+          }
+          tmem_st_x16(t_p + at / 2, w);
+        };
 #pragma unroll
         for (int i = 0; i < KEYS; i += 64) {
           tmem_ld_wait();
@@ -538,8 +544,8 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (i + 64 < KEYS) tmem_ld_x32(t_s + i + 64, r);
           weigh(other, i + 32);
         }
+        l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       }
-      l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -592,6 +598,116 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (qi < per && qq < t.queries && piece * 8 < p.dim)
             *reinterpret_cast<uint4 *>(y + qq * p.ldy + hi * p.dim + piece * 8) = *reinterpret_cast<const uint4 *>(out + rr * (DP * 2) + ((piece ^ (rr & 7)) << 4));
         }
+      }
+    }
+  } else {
+    if constexpr (Cfg::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");   // the whole group of warps, the idle ones too
+    if (warp == 4 * TILES) {
+      if (lane == 0 && n > 0) {
+        bool ok = true;
+        const int tiles = first_turn(TILES - 1) < n ? TILES : 1;
+        mbar_arrive_expect_tx(bar_q, tiles * Cfg::PANELS * 128 * p.group * per);
+        for (int x = 0; x < tiles; ++x)
+          for (int c = 0; c < Cfg::PANELS; ++c)
+            tma_load_3d(sm_q + (x * Cfg::PANELS + c) * 16384, &tm_q, bar_q, 64 * c, kh * p.group, t.q0 + x * per);
+        for (int i = 0; i < 2 * n; ++i) {   // K and V in turn
+          const uint32_t st = i % ST, ph = (i / ST) & 1;
+          const int row = t.k0 + (n - 1 - (i >> 1)) * KEYS;
+          if (!(ok = mbar_wait_relaxed(bar_empty + 8 * st, ph ^ 1u, abort_flag))) break;
+          mbar_arrive_expect_tx(bar_full + 8 * st, Cfg::TILE);
+          for (int c = 0; c < Cfg::PANELS; ++c)
+            tma_load_3d(sm_ring + st * Cfg::TILE + c * Cfg::PANEL, i & 1 ? &tm_v : &tm_k, bar_full + 8 * st, 64 * c, kh, row);
+        }
+        if (!ok) {
+          *abort_flag = 1;
+          report(p.status, DEV_WAIT_SMEM_EMPTY);
+          const uint64_t t0 = globaltimer();   // copies in flight land before the block ends
+          while (globaltimer() - t0 < 200000ull) {}
+        }
+      }
+    } else if (warp == 4 * TILES + 1) {
+      // descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, version 1
+      const uint64_t desc_hi = (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;
+      const uint32_t kmajor = 1u << 16, mnmajor = ((uint32_t)Cfg::PANEL >> 4) << 16;   // MN-major: leading offset = one panel
+      const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | (((uint32_t)KEYS >> 3) << 17) | ((128u >> 4) << 24);
+      const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
+      const uint32_t leader = lane == 0;
+      const uint32_t q_lo = kmajor | uniform(sm_q >> 4), ring = uniform(sm_ring >> 4), tm = uniform(tmem);   // below 2^14: no carry into the next field
+      const int turns = (int)uniform((uint32_t)n), visible = (int)uniform((uint32_t)lim_lo);
+      int begin[TILES];
+#pragma unroll
+      for (int x = 0; x < TILES; ++x) begin[x] = (int)uniform((uint32_t)first_turn(x));
+      bool ok = true;
+      auto scores = [&](int x, int it) -> bool {
+        const uint32_t st = (uint32_t)(2 * it) % ST, ph = ((uint32_t)(2 * it) / ST) & 1;
+        if (it >= begin[x]) {
+          if (!warp_wait(bar_full + 8 * st, ph, abort_flag)) return false;
+          tc_fence_after();
+          const uint32_t k_lo = kmajor | (ring + st * (Cfg::TILE >> 4));
+#pragma unroll
+          for (int kk = 0; kk < DP / 16; ++kk)
+            umma_ss(leader, tm + Cfg::S_COL + x * Cfg::STEP, desc_hi | (q_lo + (x * Cfg::PANELS + (kk >> 2)) * 1024 + (kk & 3) * 2),
+                    desc_hi | (k_lo + (kk >> 2) * (Cfg::PANEL >> 4) + (kk & 3) * 2), idesc_s, kk != 0);
+          commit_if(leader, bar_s + 8 * x);
+        }
+        if (x == TILES - 1) commit_if(leader, bar_empty + 8 * st);   // both tiles' products with these keys are on their way
+        return true;
+      };
+      if (turns > 0) ok = warp_wait(bar_q, 0, abort_flag);
+#pragma unroll
+      for (int x = 0; x < TILES; ++x)
+        if (turns > 0 && ok) ok = scores(x, 0);
+      for (int it = 0; it < turns && ok; ++it) {
+        const int base = (turns - 1 - it) * KEYS;
+        const uint32_t st = (uint32_t)(2 * it + 1) % ST, ph = ((uint32_t)(2 * it + 1) / ST) & 1;
+        if (Cfg::EARLY && it + 1 < turns && !(ok = warp_wait(bar_se, it & 1, abort_flag) && scores(0, it + 1))) break;
+        if (!(ok = warp_wait(bar_full + 8 * st, ph, abort_flag))) break;
+        if (base + KEYS > visible) {
+          // Values past the last key that anybody here sees belong to others and may hold anything: zeros in their place, since
+          // the tensor cores multiply every value by every row's weight and 0 * NaN is NaN.  Values on the diagonal are hidden
+          // from some rows only: if one is not finite, the rows are summed up the plain way at the end.
+          uint8_t *v = gen + Cfg::Q + st * Cfg::TILE;
+          constexpr int PIECES = 8 * Cfg::PANELS;   // 16-byte pieces of a key's values
+          const int none = max(0, min(KEYS, lim_hi - base)), some = max(0, min(none, lim_lo - base));
+          for (int i = none * PIECES + lane; i < KEYS * PIECES; i += 32) {
+            const int key = i / PIECES, piece = i % PIECES;
+            *reinterpret_cast<uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          bool bad = false;
+          for (int i = some * PIECES + lane; i < none * PIECES; i += 32) {
+            const int key = i / PIECES, piece = i % PIECES;
+            const uint4 w = *reinterpret_cast<const uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16);
+            for (uint32_t u : {w.x, w.y, w.z, w.w}) bad |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
+          }
+          if (bad) *unclean = 1;
+          fence_proxy_async();
+          __syncwarp();
+        }
+        const uint32_t v_lo = mnmajor | (ring + st * (Cfg::TILE >> 4));
+#pragma unroll
+        for (int x = 0; x < TILES; ++x) {
+          if (it >= begin[x]) {
+            if (!(ok = warp_wait(bar_p + 8 * x, (it - begin[x]) & 1, abort_flag))) break;
+            tc_fence_after();
+            const uint32_t more = it != begin[x];
+#pragma unroll
+            for (int kk = 0; kk < KEYS / 16; ++kk)   // 16 keys: 8 columns of P, 16 rows of V
+              umma_ts(leader, tm + Cfg::O_COL + x * Cfg::STEP, tm + Cfg::P_COL + x * Cfg::STEP + 8 * kk, desc_hi | (v_lo + 128 * kk), idesc_o,
+                      kk != 0 ? 1u : more);
+          }
+          if (x == TILES - 1) commit_if(leader, bar_empty + 8 * st);
+          if (it + 1 == turns && begin[x] < turns) {
+            commit_if(leader, bar_o + 8 * x);
+            if (lane == 0) mbar_arrive(bar_o + 8 * x);
+          }
+          // Without columns of their own the weights lie where the next scores go.  Both products are this thread's, and the
+          // tensor cores take them in order.
+          if (!Cfg::EARLY && it + 1 < turns && !(ok = scores(x, it + 1))) break;
+        }
+      }
+      if (!ok && lane == 0) {
+        *abort_flag = 1;
+        report(p.status, DEV_WAIT_SMEM_FULL);
       }
     }
   }
