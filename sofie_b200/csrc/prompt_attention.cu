@@ -9,7 +9,6 @@
 #include <math.h>
 #include <mutex>
 #include <new>
-#include <type_traits>
 
 #include "generate.cuh"
 #include "ptx.cuh"
@@ -32,60 +31,87 @@ struct PromptParams {
 // One tile of queries: its sequence's rows, its first query and how many of them there are.
 struct PromptTile {
   int q0, k0, k_len;      // first query row of the tile and first key row of the sequence in the packed tensors; keys of the sequence
-  int queries;            // 0: nothing to do
+  int queries;            // 0: no such tile; -1 (in a block's mail): no more tiles
   int past;               // keys that the tile's first query sees, before clamping to [0, k_len] (causal)
+  int kh;                 // key head
 };
 
-// Tiles are counted sequence by sequence; within a sequence the last one, which sees most keys, comes first.  All threads call
-// it (THREADS of them); each sums up a few neighbouring sequences.
-template <int THREADS>
-__device__ __forceinline__ PromptTile find_tile(const PromptParams &p, int index) {
-  __shared__ long long warp_sum[THREADS / 32];
-  __shared__ PromptTile s_tile;
+// Sequence b: tiles of `tokens` queries; fills in the parts of t that are the sequence's.
+__device__ __forceinline__ int sequence_tiles(const PromptParams &p, int b, PromptTile &t, int &q_len) {
+  int x0, x1, y0, y1;
+  bool bad = false;
+  packed_range(p.cu_q, b, p.q_rows, &x0, &x1, &bad);
+  packed_range(p.cu_k, b, p.k_rows, &y0, &y1, &bad);
+  if (bad) report(p.status, DEV_BAD_INDEX);
+  t.q0 = x0; t.k0 = y0; t.k_len = y1 - y0;
+  q_len = bad ? 0 : x1 - x0;
+  return (q_len + p.tokens - 1) / p.tokens;
+}
+
+// Tiles are counted sequence by sequence; within a sequence the last one, which sees most keys, comes first.  The table of a block
+// has the tiles before each of RUNS equal runs of sequences.  All threads call this, at least RUNS of them.
+constexpr int RUNS = 128;
+__device__ __forceinline__ void count_tiles(const PromptParams &p, int *table) {   // [RUNS + 1]
+  __shared__ long long warp_sum[RUNS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (p.batch + THREADS - 1) / THREADS;
-  const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
-  auto tiles_of = [&](int b, PromptTile &t, int &q_len) -> int {
-    int x0, x1, y0, y1;
-    bool bad = false;
-    packed_range(p.cu_q, b, p.q_rows, &x0, &x1, &bad);
-    packed_range(p.cu_k, b, p.k_rows, &y0, &y1, &bad);
-    if (bad) report(p.status, DEV_BAD_INDEX);
-    t.q0 = x0; t.k0 = y0; t.k_len = y1 - y0;
-    q_len = bad ? 0 : x1 - x0;
-    return (q_len + p.tokens - 1) / p.tokens;
-  };
+  const int per = (p.batch + RUNS - 1) / RUNS;
+  const int b0 = tid < RUNS ? min(p.batch, tid * per) : p.batch, b1 = min(p.batch, b0 + per);
   PromptTile t;
   int q_len;
   long long mine = 0;   // offsets that claim rows twice can make more tiles than the grid has; the rest is left out
-  for (int b = b0; b < b1; ++b) mine += tiles_of(b, t, q_len);
+  for (int b = b0; b < b1; ++b) mine += sequence_tiles(p, b, t, q_len);
   long long incl = mine;
   for (int o = 1; o < 32; o <<= 1) {
     const long long x = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += x;
   }
-  if (lane == 31) warp_sum[warp] = incl;
-  if (tid == 0) s_tile.queries = 0;
+  if (lane == 31 && tid < RUNS) warp_sum[warp] = incl;
   __syncthreads();
-  long long before = incl - mine;
-  for (int w = 0; w < warp; ++w) before += warp_sum[w];
-  if (index >= before && index < before + mine) {
-    long long at = before;
-    for (int b = b0; b < b1; ++b) {
-      const int n = tiles_of(b, t, q_len);
-      if (index < at + n) {
-        const int first = (n - 1 - (int)(index - at)) * p.tokens;
-        t.past = first + 1 + t.k_len - q_len;
-        t.q0 += first;
-        t.queries = min(p.tokens, q_len - first);
-        s_tile = t;
-        break;
-      }
-      at += n;
-    }
+  if (tid < RUNS) {
+    for (int w = 0; w < warp; ++w) incl += warp_sum[w];
+    if (tid == 0) table[0] = 0;
+    table[tid + 1] = (int)min(incl, 0x7fffffffLL);
   }
   __syncthreads();
-  return s_tile;
+}
+
+// Tile `index` for all lanes of a warp; queries = 0 when there is none.
+__device__ __forceinline__ PromptTile find_tile(const PromptParams &p, const int *table, int index) {
+  const int lane = threadIdx.x & 31;
+  PromptTile t{};
+  if (index >= table[RUNS]) return t;
+  int run = 0;   // runs that end at or before the index
+#pragma unroll
+  for (int i = 0; i < RUNS; i += 32) run += __popc(__ballot_sync(0xffffffffu, table[i + lane + 1] <= index));
+  const int per = (p.batch + RUNS - 1) / RUNS;
+  const int b1 = min(p.batch, (run + 1) * per);
+  int at = table[run];
+  for (int b = run * per; b < b1; b += 32) {
+    int q_len = 0;
+    const int n = b + lane < b1 ? sequence_tiles(p, b + lane, t, q_len) : 0;
+    int incl = n;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const bool here = index >= at + incl - n && index < at + incl;
+    const uint32_t who = __ballot_sync(0xffffffffu, here);
+    if (who) {
+      const int first = (n - 1 - (index - (at + incl - n))) * p.tokens;
+      t.past = first + 1 + t.k_len - q_len;
+      t.q0 += first;
+      t.queries = min(p.tokens, q_len - first);
+      const int src = __ffs(who) - 1;
+      t.q0 = __shfl_sync(0xffffffffu, t.q0, src);
+      t.k0 = __shfl_sync(0xffffffffu, t.k0, src);
+      t.k_len = __shfl_sync(0xffffffffu, t.k_len, src);
+      t.queries = __shfl_sync(0xffffffffu, t.queries, src);
+      t.past = __shfl_sync(0xffffffffu, t.past, src);
+      return t;
+    }
+    at += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return PromptTile{};
 }
 
 // Keys that query i of the tile sees.
@@ -155,6 +181,11 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
 
+// The same for waits that are usually long: sleeps between polls.
+__device__ __forceinline__ bool warp_wait_long(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait_relaxed(bar, parity, abort_flag));
+}
+
 // ---- bf16 on the tensor cores --------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -167,26 +198,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
-// 2^x for x <= 2^7 on the FMA pipes: the special-function unit does 16 exponentials a cycle and SM, as long for a tile's scores as the
-// tensor cores need for both products, so some of them go another way.  x = n + r with n the nearest integer (x + 1.5 * 2^23
-// leaves n in the low bits), 2^r on [-1/2, 1/2] by the polynomial of degree 4 with p(0) = 1 whose largest relative error is
-// least (2.9e-6, fitted to 2^r by linear programming), n added to the exponent.  Below -127 the result is 0, as ex2 flushes.
-__device__ __forceinline__ float2 exp2_pair(float2 x) {
-  x.x = fmaxf(x.x, -127.f);
-  x.y = fmaxf(x.y, -127.f);
-  const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));
-  const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
-  const float2 r = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
-  float2 p = __ffma2_rn(r, make_float2(0.0095828529f, 0.0095828529f), make_float2(0.0559064262f, 0.0559064262f));
-  p = __ffma2_rn(p, r, make_float2(0.2402409911f, 0.2402409911f));
-  p = __ffma2_rn(p, r, make_float2(0.6931241751f, 0.6931241751f));
-  p = __ffma2_rn(p, r, make_float2(1.f, 1.f));
-  return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
-}
-#ifndef SB_POLY
-#define SB_POLY 0x8888u
-#endif
-constexpr uint32_t POLY = SB_POLY;   // of 16 pairs, those that exp2_pair takes
 // The issuing warp stays together and one lane's predicate does the rest: the operands are then the same in every lane, which
 // lets the compiler keep them in uniform registers.  With a branch to one lane around the products every operand was moved there
 // one by one, and issuing a tile's 16 products took longer than computing them.
@@ -224,29 +235,29 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t *r) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A block computes TILES tiles of 128 rows against the same keys and values.  What sets the sizes is the way from L2: a tile of keys
+// A block works on TILES tiles of 128 rows against the same keys and values.  What sets the sizes is the way from L2: a tile of keys
 // and values takes about 3000 cycles from request to arrival and an SM sustains about 48 bytes per cycle, while the tensor cores
 // would finish 128 rows x 128 keys of head size 128 (64 KB of keys and values) in 1024 cycles.  So at that head size two tiles of rows
 // share every load (32 bytes per cycle at full rate) and five tiles of keys or values are in flight; at head size 64 half the bytes
-// are needed per score, and two blocks of one tile share an SM instead, one's beginning and end beside the other's middle.
+// are needed per score, and two blocks of one tile share an SM instead.
 template <int DP>
 struct UmmaCfg;
 template <>
 struct UmmaCfg<64> {
-  static constexpr int TILES = 1, KEYS = 128, BLOCKS = 2, STAGES = 5, COLS = 256;
+  static constexpr int TILES = 1, KEYS = 128, BLOCKS = 2, STAGES = 4, QS = 2, COLS = 256;
   static constexpr int S_COL = 0, O_COL = 128, P_COL = 192, STEP = 0;
   static constexpr bool EARLY = true;    // the weights have columns of their own: the next scores are computed meanwhile
   static constexpr bool HOLD = false;    // a thread holds its whole row of scores in registers
 };
 template <>
 struct UmmaCfg<128> {
-  static constexpr int TILES = 2, KEYS = 128, BLOCKS = 1, STAGES = 5, COLS = 512;
+  static constexpr int TILES = 2, KEYS = 128, BLOCKS = 1, STAGES = 5, QS = 1, COLS = 512;
   static constexpr int S_COL = 0, O_COL = 128, P_COL = 0, STEP = 256;
   static constexpr bool EARLY = false, HOLD = true;
 };
 template <>
 struct UmmaCfg<256> {
-  static constexpr int TILES = 1, KEYS = 64, BLOCKS = 1, STAGES = 5, COLS = 512;
+  static constexpr int TILES = 1, KEYS = 64, BLOCKS = 1, STAGES = 5, QS = 1, COLS = 512;
   static constexpr int S_COL = 0, O_COL = 256, P_COL = 64, STEP = 0;
   static constexpr bool EARLY = true, HOLD = true;
 };
@@ -261,8 +272,31 @@ struct UmmaSize : UmmaCfg<DP> {
   // is launched with a whole third group of warps, which hands registers over, 384 x 168 = 256 x 216 + 128 x 72.
   static constexpr bool MOVE = C::TILES == 2;
   static constexpr int THREADS = C::TILES * 128 + (MOVE ? 128 : 64);
-  static constexpr int SMEM = Q + C::STAGES * TILE + 1024 /*barriers*/ + 1024 /*alignment*/;
+  static constexpr int CONTROL = 512 + 64 + 64 + 4 * (RUNS + 1);   // barriers, mail, answers, table of tiles
+  static constexpr int SMEM = C::QS * Q + C::STAGES * TILE + (CONTROL + 127) / 128 * 128 + 1024 /*alignment*/;
 };
+
+// The next tile of a block whose first one is blockIdx.x: the hardware hands over a block of the grid that has not begun (cluster
+// launch control), so tiles go to whoever is free, the heavy ones first, without a counter in memory that two graphs could share.
+__device__ __forceinline__ void ask_for_block(uint32_t answer, uint32_t bar) {
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer), "r"(bar) : "memory");
+}
+__device__ __forceinline__ bool block_given(uint32_t answer, uint32_t &index) {
+  uint32_t given, x = 0;
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b128 h;\n"
+      "ld.shared.b128 h, [%2];\n"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "mov.u32 %1, 0;\n"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, h;\n}\n"
+      : "=r"(given), "=r"(x)
+      : "r"(answer)
+      : "memory");
+  index = x;
+  return given != 0;
+}
 
 // The plain sum for one row, from global memory.  Taken when values that some rows of a tile do not see hold NaN or infinities: the
 // tensor cores multiply every value by every row's weight, and 0 * NaN would reach rows it must not reach.
@@ -293,50 +327,58 @@ __device__ __noinline__ void plain_row(const PromptParams &p, long long q_row, i
   }
 }
 
-// Roles:
-//   a warp, lane 0   TMA: the queries once, then per tile of keys K and V, from the last tile to the first, into a ring
+// Blocks stay and take tile after tile.  Roles:
+//   a warp           finds the tile, leaves it in the mail for the others, asks for the next; lane 0 loads by TMA: the queries once, then
+//                    per tile of keys K and V, from the last to the first, into a ring -- of the next tile while this one is computed
 //   a warp           MMA: S = Q K^T (operands in shared memory), O += P V (P in tensor memory, V MN-major in shared memory)
-//   4 warps a tile   a thread per row: maximum, exponentials, row sum; P as bf16 back to tensor memory
+//   4 warps a tile   a thread per row: maximum, exponentials, row sum; P as bf16 back to tensor memory, in two halves, the first of which
+//                    is multiplied while the second is computed
 // The reference maximum of a row moves only when a tile's maximum is 2^8 above it (weights stay below 2^8, exact in effect
 // since numerator and denominator use the same); then O is rescaled in tensor memory, which after the first tiles is rare.
-// Only tiles that the sequence's end or the diagonal cross pay for masks.
+// Only tiles that the sequence's end or the diagonal cross pay for masks.  Every wait has a limit.
 template <int DP>
 __global__ void __launch_bounds__(UmmaSize<DP>::THREADS, UmmaSize<DP>::BLOCKS)
 prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                    const __grid_constant__ PromptParams p) {
   using Cfg = UmmaSize<DP>;
-  constexpr int ST = Cfg::STAGES, KEYS = Cfg::KEYS, TILES = Cfg::TILES;
+  constexpr int ST = Cfg::STAGES, KEYS = Cfg::KEYS, TILES = Cfg::TILES, QS = Cfg::QS;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), pad = (1024u - (raw & 1023u)) & 1023u;
-  const uint32_t sm_q = raw + pad, sm_ring = sm_q + Cfg::Q;
+  const uint32_t sm_q = raw + pad, sm_ring = sm_q + QS * Cfg::Q;
   uint8_t *gen = smem_raw + pad;
-  uint8_t *tail = gen + Cfg::Q + ST * Cfg::TILE;
-  const uint32_t bar_q = smem_u32(tail);             // queries landed
-  const uint32_t bar_full = bar_q + 8;               // [ST] ring: keys or values landed
+  uint8_t *tail = gen + QS * Cfg::Q + ST * Cfg::TILE;
+  const uint32_t bar_mail = smem_u32(tail);          // [2] a tile is in the mail
+  const uint32_t bar_read = bar_mail + 16;           // [2] everybody has read it
+  const uint32_t bar_next = bar_read + 16;           // [2] the answer about the next tile is there
+  const uint32_t bar_q = bar_next + 16;              // [QS] queries landed
+  const uint32_t bar_qe = bar_q + 8 * QS;            // [QS] queries read
+  const uint32_t bar_full = bar_qe + 8 * QS;         // [ST] ring: keys or values landed
   const uint32_t bar_empty = bar_full + 8 * ST;      // [ST] the products that read them are complete
   const uint32_t bar_s = bar_empty + 8 * ST;         // [TILES] scores complete in tensor memory
   const uint32_t bar_se = bar_s + 8 * TILES;         // [TILES] scores read (EARLY)
-  const uint32_t bar_p = bar_se + 8 * TILES;         // [TILES] weights written to tensor memory
-  const uint32_t bar_o = bar_p + 8 * TILES;          // [TILES] result complete
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 512);
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + 516);
-  volatile int *unclean = reinterpret_cast<volatile int *>(tail + 520);   // non-finite values where the mask hides some of them
+  const uint32_t bar_p = bar_se + 8 * TILES;         // [TILES][2] half of the weights written to tensor memory
+  const uint32_t bar_pv = bar_p + 16 * TILES;        // [TILES] product with the values complete (EARLY)
+  const uint32_t bar_o = bar_pv + 8 * TILES;         // [TILES] result complete
+  const uint32_t bar_oe = bar_o + 8 * TILES;         // [TILES] result read
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 448);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tail + 452);
+  volatile int *unclean = reinterpret_cast<volatile int *>(tail + 456);   // [4] 1 + number of a tile with non-finite values where the mask hides some
+  PromptTile *mail = reinterpret_cast<PromptTile *>(tail + 512);          // [2]
+  const uint32_t answer = smem_u32(tail + 576);                           // [2] 16 bytes
+  int *table = reinterpret_cast<int *>(tail + 640);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  const int kh = blockIdx.x % p.kv_heads;
-  const PromptTile t = find_tile<Cfg::THREADS>(p, blockIdx.x / p.kv_heads);
-  if (t.queries == 0) return;
-  const int per = 128 / p.group;                                           // queries of a tile of rows
-  const int lim_lo = seen(p, t, 0), lim_hi = seen(p, t, t.queries - 1);   // keys that the first and the last query see
-  const int n = (lim_hi + KEYS - 1) / KEYS;                                // tiles of keys; they are taken from the last to the first
-  // a tile of rows whose last query sees fewer keys starts later; one without queries has no turn
-  auto first_turn = [&](int x) {
-    const int have = min(per, t.queries - x * per);
-    return have <= 0 ? n : n - (seen(p, t, x * per + have - 1) + KEYS - 1) / KEYS;
-  };
+  const int per = 128 / p.group;                                          // queries of a tile of rows
 
   if (tid == 0) {
-    mbar_init(bar_q, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar_mail + 8 * i, 1);
+      mbar_init(bar_read + 8 * i, 4 * TILES + 1);
+      mbar_init(bar_next + 8 * i, 1);
+    }
+    for (int i = 0; i < QS; ++i) {
+      mbar_init(bar_q + 8 * i, 1);
+      mbar_init(bar_qe + 8 * i, 1);
+    }
     for (int s = 0; s < ST; ++s) {
       mbar_init(bar_full + 8 * s, 1);
       mbar_init(bar_empty + 8 * s, 1);
@@ -344,286 +386,362 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     for (int x = 0; x < TILES; ++x) {
       mbar_init(bar_s + 8 * x, 1);
       mbar_init(bar_se + 8 * x, 4);
-      mbar_init(bar_p + 8 * x, 4);
+      mbar_init(bar_p + 16 * x, 4);
+      mbar_init(bar_p + 16 * x + 8, 4);
+      mbar_init(bar_pv + 8 * x, 1);
       mbar_init(bar_o + 8 * x, 2);   // the product, and the issuer's word on `unclean`
+      mbar_init(bar_oe + 8 * x, 4);
     }
     *abort_flag = 0;
-    *unclean = 0;
+    for (int i = 0; i < 4; ++i) unclean[i] = 0;
     fence_barrier_init();
+    prefetch_tensormap(&tm_q);
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
   }
   if (warp == 4 * TILES + 1) {
     tmem_alloc(smem_u32(tmem_slot), Cfg::COLS);
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  count_tiles(p, table);   // ends with a barrier of the block
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+
+  // The i-th tile of the block from the mail, for the warps that compute.
+  auto receive = [&](int i, PromptTile &t) -> bool {
+    if (!warp_wait(bar_mail + 8 * (i & 1), (i >> 1) & 1, abort_flag)) return false;
+    t = mail[i & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_read + 8 * (i & 1));
+    return true;
+  };
+  // Tiles of keys are taken from the last to the first.  A tile of rows whose last query sees fewer keys starts later; one without
+  // queries or keys has no turn.
+  auto first_turn = [&](const PromptTile &t, int n, int x) {
+    const int have = min(per, t.queries - x * per);
+    return have <= 0 ? n : n - (seen(p, t, x * per + have - 1) + KEYS - 1) / KEYS;
+  };
 
   if (warp < 4 * TILES) {
     if constexpr (Cfg::MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     const int x = warp >> 2;                      // tile of rows
     const int row = (warp & 3) * 32 + lane;
     const int in_tile = row / p.group, head = row - in_tile * p.group, query = x * per + in_tile;
-    const bool mine = in_tile < per && query < t.queries;   // rows past the last query (and past per * group) hold anything
-    const int lim = mine ? seen(p, t, query) : lim_hi;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lanes + Cfg::S_COL + x * Cfg::STEP, t_p = tmem + lanes + Cfg::P_COL + x * Cfg::STEP;
     const uint32_t t_o = tmem + lanes + Cfg::O_COL + x * Cfg::STEP;
     const float c = p.scale_log2e;
-    float m = -INFINITY, l = 0.f;   // reference maximum of the unscaled scores; sum of the weights
-    const int begin = first_turn(x);
-    // a tile's maximum: moves the reference maximum if it has to, and with it the sum and O
-    auto raise = [&](float top, int turn) {
-      if (turn == 0) {
-        m = top;
-        return;
-      }
-      const bool up = (top - m) * c > 8.f;
-      if (!__any_sync(0xffffffffu, up)) return;
-      const float f = up ? ex2((m - top) * c) : 1.f;
-      if (up) m = top;
-      l *= f;
-#pragma unroll
-      for (int d = 0; d < DP; d += 16) {
-        uint32_t o[16];
-        tmem_ld_x16(t_o + d, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-        tmem_st_x16(t_o + d, o);
-      }
-    };
+    const float2 c2 = make_float2(c, c);
+    const bool sectors = p.dim % 16 == 0 && p.ldy % 16 == 0 && ((uintptr_t)p.y & 31) == 0;
+    uint32_t turns = 0, results = 0;   // of this tile of rows so far: the parities of its barriers
+    PromptTile t;
     bool ok = true;
-    for (int it = begin; it < n; ++it) {
-      const int base = (n - 1 - it) * KEYS, turn = it - begin;
-      if (!(ok = warp_wait(bar_s + 8 * x, turn & 1, abort_flag))) break;
-      tc_fence_after();
-      const int have = lim - base;   // keys of this tile that the row sees
-      const bool masked = base + KEYS > lim_lo;
-      const float2 c2 = make_float2(c, c);
-      bool careful = masked || turn == 0;
-      if constexpr (Cfg::HOLD) {
-        uint32_t r[KEYS];
-        float *s = reinterpret_cast<float *>(r);
-#pragma unroll
-        for (int i = 0; i < KEYS; i += 32) tmem_ld_x32(t_s + i, r + i);
-        tmem_ld_wait();
-        if (Cfg::EARLY) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_se + 8 * x);
-          if (turn > 0) {   // the previous product has left P and O
-            const int i = 2 * it - 1;
-            if (!(ok = warp_wait(bar_empty + 8 * (i % ST), (i / ST) & 1, abort_flag))) break;
-            tc_fence_after();
-          }
+    for (int i = 0; ok && (ok = receive(i, t)) && t.queries > 0; ++i) {
+      if (x * per >= t.queries) continue;
+      const int lim_lo = seen(p, t, 0), lim_hi = seen(p, t, t.queries - 1);   // keys that the first and the last query see
+      const int n = (lim_hi + KEYS - 1) / KEYS, begin = first_turn(t, n, x);
+      const bool mine = in_tile < per && query < t.queries;   // rows past the last query (and past per * group) hold anything
+      const int lim = mine ? seen(p, t, query) : lim_hi;
+      float m = -INFINITY, l = 0.f;   // reference maximum of the unscaled scores; sum of the weights
+      // a tile's maximum: moves the reference maximum if it has to, and with it the sum and O
+      auto raise = [&](float top, bool first) {
+        if (first) {
+          m = top;
+          return;
         }
-        // 32 scores -> 16 columns of P.  MIX: the pairs of each 16 whose exponentials are a polynomial (see exp2_pair).
-        auto weigh = [&](int at, float2 off2, float2 &sum, auto mix) {
-          constexpr uint32_t MIX = decltype(mix)::value;
-          uint32_t w[16];
-          float2 other = make_float2(0.f, 0.f);
+        const bool up = (top - m) * c > 8.f;
+        if (!__any_sync(0xffffffffu, up)) return;
+        const float f = up ? ex2((m - top) * c) : 1.f;
+        if (up) m = top;
+        l *= f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 e = __ffma2_rn(make_float2(s[at + 2 * i], s[at + 2 * i + 1]), c2, off2);
-            if ((MIX >> i) & 1) {
-              e = exp2_pair(e);
-            } else {
+        for (int d = 0; d < DP; d += 16) {
+          uint32_t o[16];
+          tmem_ld_x16(t_o + d, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+          tmem_st_x16(t_o + d, o);
+        }
+      };
+      auto hand_over = [&](int half) {   // half of P is in tensor memory
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_p + 16 * x + 8 * half);
+      };
+      for (int it = begin; it < n; ++it, ++turns) {
+        const int base = (n - 1 - it) * KEYS;
+        if (!(ok = warp_wait(bar_s + 8 * x, turns & 1, abort_flag))) break;
+        tc_fence_after();
+        const int have = lim - base;   // keys of this tile that the row sees
+        const bool masked = base + KEYS > lim_lo, first = it == begin;
+        if constexpr (Cfg::HOLD) {
+          uint32_t r[KEYS];
+          float *s = reinterpret_cast<float *>(r);
+#pragma unroll
+          for (int k = 0; k < KEYS; k += 32) tmem_ld_x32(t_s + k, r + k);
+          tmem_ld_wait();
+          if (Cfg::EARLY) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_se + 8 * x);
+            if (!first) {   // the previous product has left P and O
+              if (!(ok = warp_wait(bar_pv + 8 * x, (turns - 1) & 1, abort_flag))) break;
+              tc_fence_after();
+            }
+          }
+          auto weigh = [&](int at, float2 off2, float2 &sum) {   // 32 scores -> 16 columns of P
+            uint32_t w[16];
+            float2 other = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float2 e = __ffma2_rn(make_float2(s[at + 2 * k], s[at + 2 * k + 1]), c2, off2);
               e.x = ex2(e.x);
               e.y = ex2(e.y);
+              if (k & 1) other = __fadd2_rn(other, e);
+              else sum = __fadd2_rn(sum, e);
+              const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
+              w[k] = *reinterpret_cast<const uint32_t *>(&h);
             }
-            if (i & 1) other = __fadd2_rn(other, e);
-            else sum = __fadd2_rn(sum, e);
-            const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
-            w[i] = *reinterpret_cast<const uint32_t *>(&h);
-          }
-          sum = __fadd2_rn(sum, other);
-          tmem_st_x16(t_p + at / 2, w);
-        };
-        if (!careful) {
-          // The weights by the reference maximum that is there, without waiting for this tile's own; that one is found beside
-          // them and, if it is more than 2^8 above (or a score is NaN or +inf), the tile is done over.
-          const float off = -m * c;
-          float2 sum = make_float2(0.f, 0.f);
-          float x0 = s[0], x1 = s[1];
+            sum = __fadd2_rn(sum, other);
+            tmem_st_x16(t_p + at / 2, w);
+          };
+          bool careful = masked || first;
+          if (!careful) {
+            // The weights by the reference maximum that is there, without waiting for this tile's own; that one is found beside
+            // the first half and, if it is more than 2^8 above (or a score is NaN or +inf), the tile is done over.
+            const float off = -m * c;
+            float2 sum = make_float2(0.f, 0.f);
+            float x0 = s[0], x1 = s[1];
 #pragma unroll
-          for (int i = 0; i < KEYS; i += 32) {
-            weigh(i, make_float2(off, off), sum, std::integral_constant<uint32_t, POLY>());
+            for (int k = 0; k < KEYS / 2; k += 32) {
+              weigh(k, make_float2(off, off), sum);
 #pragma unroll
-            for (int k = i; k < i + 32; k += 4) {
-              x0 = max3_nan(x0, s[k], s[k + 1]);
-              x1 = max3_nan(x1, s[k + 2], s[k + 3]);
+              for (int e = 2 * k; e < 2 * k + 64; e += 4) {
+                x0 = max3_nan(x0, s[e], s[e + 1]);
+                x1 = max3_nan(x1, s[e + 2], s[e + 3]);
+              }
+            }
+            const float top = max3_nan(x0, x1, x1);
+            careful = __any_sync(0xffffffffu, mine && !((top - m) * c <= 8.f));
+            if (!careful) {
+              hand_over(0);
+#pragma unroll
+              for (int k = KEYS / 2; k < KEYS; k += 32) weigh(k, make_float2(off, off), sum);
+              l += sum.x + sum.y;
             }
           }
-          const float top = max3_nan(x0, x1, x1);
-          careful = __any_sync(0xffffffffu, mine && !((top - m) * c <= 8.f));
-          if (!careful) l += sum.x + sum.y;
-        }
-        if (careful) {
-          tmem_st_wait();   // what the first attempt wrote is written again
-          if (masked)
+          if (careful) {
+            tmem_st_wait();   // what the first attempt wrote is written again
+            if (masked)
 #pragma unroll
-            for (int i = 0; i < KEYS; ++i) s[i] = i < have ? s[i] : -INFINITY;
-          float x0 = s[0], x1 = s[1];
+              for (int k = 0; k < KEYS; ++k) s[k] = k < have ? s[k] : -INFINITY;
+            float x0 = s[0], x1 = s[1];
 #pragma unroll
-          for (int i = 2; i < KEYS; i += 2) {
-            x0 = fmaxf(x0, s[i]);
-            x1 = fmaxf(x1, s[i + 1]);
+            for (int k = 2; k < KEYS; k += 2) {
+              x0 = fmaxf(x0, s[k]);
+              x1 = fmaxf(x1, s[k + 1]);
+            }
+            raise(fmaxf(x0, x1), first);
+            const float off = m == -INFINITY ? 0.f : -m * c;
+            float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < KEYS; k += 32) weigh(k, make_float2(off, off), sum);
+            l += sum.x + sum.y;
+            hand_over(0);
           }
-          raise(fmaxf(x0, x1), turn);
+          hand_over(1);
+        } else {
+          // twice from tensor memory, 32 columns at a time: once for the maximum, once for the weights
+          uint32_t r[32], other[32];
+          float top = -INFINITY;
+          auto take = [&](uint32_t *w, int at) {
+            float *s = reinterpret_cast<float *>(w);
+            if (masked)
+#pragma unroll
+              for (int k = 0; k < 32; ++k) s[k] = at + k < have ? s[k] : -INFINITY;
+            float x0 = s[0], x1 = s[1];
+#pragma unroll
+            for (int k = 2; k < 32; k += 2) {
+              x0 = fmaxf(x0, s[k]);
+              x1 = fmaxf(x1, s[k + 1]);
+            }
+            top = fmaxf(top, fmaxf(x0, x1));
+          };
+#pragma unroll
+          for (int k = 0; k < KEYS; k += 64) {
+            if (k == 0) tmem_ld_x32(t_s, r);
+            tmem_ld_wait();
+            tmem_ld_x32(t_s + k + 32, other);
+            take(r, k);
+            tmem_ld_wait();
+            if (k + 64 < KEYS) tmem_ld_x32(t_s + k + 64, r);
+            take(other, k + 32);
+          }
+          if (Cfg::EARLY && !first) {   // the previous product has left P and O
+            if (!(ok = warp_wait(bar_pv + 8 * x, (turns - 1) & 1, abort_flag))) break;
+            tc_fence_after();
+          }
+          raise(top, first);
+          tmem_ld_x32(t_s, r);
           const float off = m == -INFINITY ? 0.f : -m * c;
-          float2 sum = make_float2(0.f, 0.f);
+          const float2 off2 = make_float2(off, off);
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+          auto weigh = [&](const uint32_t *from, int at) {
+            const float *s = reinterpret_cast<const float *>(from);
+            uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < KEYS; i += 32) weigh(i, make_float2(off, off), sum, std::integral_constant<uint32_t, 0>());
-          l += sum.x + sum.y;
-        }
-      } else {
-        // twice from tensor memory, 32 columns at a time: once for the maximum, once for the weights
-        uint32_t r[32], other[32];
-        float top = -INFINITY;
-        auto take = [&](uint32_t *w, int at) {
-          float *s = reinterpret_cast<float *>(w);
-          if (masked)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) s[i] = at + i < have ? s[i] : -INFINITY;
-          float x0 = s[0], x1 = s[1];
-#pragma unroll
-          for (int i = 2; i < 32; i += 2) {
-            x0 = fmaxf(x0, s[i]);
-            x1 = fmaxf(x1, s[i + 1]);
-          }
-          top = fmaxf(top, fmaxf(x0, x1));
-        };
-#pragma unroll
-        for (int i = 0; i < KEYS; i += 64) {
-          if (i == 0) tmem_ld_x32(t_s, r);
-          tmem_ld_wait();
-          tmem_ld_x32(t_s + i + 32, other);
-          take(r, i);
-          tmem_ld_wait();
-          if (i + 64 < KEYS) tmem_ld_x32(t_s + i + 64, r);
-          take(other, i + 32);
-        }
-        if (Cfg::EARLY && turn > 0) {
-          const int i = 2 * it - 1;
-          if (!(ok = warp_wait(bar_empty + 8 * (i % ST), (i / ST) & 1, abort_flag))) break;
-          tc_fence_after();
-        }
-        raise(top, turn);
-        tmem_ld_x32(t_s, r);
-        const float off = m == -INFINITY ? 0.f : -m * c;
-        const float2 off2 = make_float2(off, off);
-        float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-        auto weigh = [&](const uint32_t *from, int at) {
-          const float *s = reinterpret_cast<const float *>(from);
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float2 e = make_float2(s[2 * i], s[2 * i + 1]);
-            if (masked) {
-              e.x = at + 2 * i < have ? e.x : -INFINITY;
-              e.y = at + 2 * i + 1 < have ? e.y : -INFINITY;
+            for (int k = 0; k < 16; ++k) {
+              float2 e = make_float2(s[2 * k], s[2 * k + 1]);
+              if (masked) {
+                e.x = at + 2 * k < have ? e.x : -INFINITY;
+                e.y = at + 2 * k + 1 < have ? e.y : -INFINITY;
+              }
+              e = __ffma2_rn(e, c2, off2);
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              if (k & 1) sum1 = __fadd2_rn(sum1, e);
+              else sum0 = __fadd2_rn(sum0, e);
+              const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
+              w[k] = *reinterpret_cast<const uint32_t *>(&h);
             }
-            e = __ffma2_rn(e, c2, off2);
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            if (i & 1) sum1 = __fadd2_rn(sum1, e);
-            else sum0 = __fadd2_rn(sum0, e);
-            const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
-            w[i] = *reinterpret_cast<const uint32_t *>(&h);
-          }
-          tmem_st_x16(t_p + at / 2, w);
-        };
+            tmem_st_x16(t_p + at / 2, w);
+          };
 #pragma unroll
-        for (int i = 0; i < KEYS; i += 64) {
-          tmem_ld_wait();
-          tmem_ld_x32(t_s + i + 32, other);
-          weigh(r, i);
-          tmem_ld_wait();
-          if (i + 64 < KEYS) tmem_ld_x32(t_s + i + 64, r);
-          weigh(other, i + 32);
+          for (int k = 0; k < KEYS; k += 64) {
+            tmem_ld_wait();
+            tmem_ld_x32(t_s + k + 32, other);
+            weigh(r, k);
+            tmem_ld_wait();
+            if (k + 64 < KEYS) {
+              tmem_ld_x32(t_s + k + 64, r);
+            } else if (Cfg::EARLY) {   // the scores are read
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar_se + 8 * x);
+            }
+            weigh(other, k + 32);
+            if (k + 64 == KEYS / 2) hand_over(0);
+          }
+          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+          hand_over(1);
         }
-        l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (Cfg::EARLY && !Cfg::HOLD) mbar_arrive(bar_se + 8 * x);
-        mbar_arrive(bar_p + 8 * x);
+      if (!ok) break;
+      const long long q_row = (long long)t.q0 + query;
+      const int all_heads = t.kh * p.group + head;
+      bool plain = false;
+      if (begin < n) {
+        if (!(ok = warp_wait(bar_o + 8 * x, results & 1, abort_flag))) break;
+        ++results;
+        tc_fence_after();
+        plain = unclean[i & 3] == i + 1;
       }
+      const float inv = 1.f / l;
+      const bool none = begin == n || lim <= 0;
+      __nv_bfloat16 *y = static_cast<__nv_bfloat16 *>(p.y) + q_row * p.ldy + (long long)all_heads * p.dim;
+#pragma unroll
+      for (int d = 0; d < DP; d += 32) {
+        uint32_t o[32];
+        if (begin < n) {
+          tmem_ld_x32(t_o + d, o);
+          tmem_ld_wait();
+          if (d + 32 == DP) {   // the next tile's products may begin
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_oe + 8 * x);
+          }
+        }
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const __nv_bfloat162 h = none ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
+          w[k] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+        if (!mine || plain) continue;
+        if (sectors) {   // a lane's row leaves in whole 32-byte sectors
+#pragma unroll
+          for (int k = 0; k < 16; k += 8)
+            if (d + 2 * k < p.dim)
+              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(y + d + 2 * k), "r"(w[k]), "r"(w[k + 1]), "r"(w[k + 2]), "r"(w[k + 3]),
+                           "r"(w[k + 4]), "r"(w[k + 5]), "r"(w[k + 6]), "r"(w[k + 7])
+                           : "memory");
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; k += 4)
+            if (d + 2 * k < p.dim) *reinterpret_cast<uint4 *>(y + d + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+        }
+      }
+      if (plain && mine) plain_row(p, q_row, all_heads, t.k0, lim);
     }
-    if (ok && begin < n) ok = warp_wait(bar_o + 8 * x, 0, abort_flag);
     if (!ok) {
       *abort_flag = 1;
       report(p.status, DEV_WAIT_TMEM_FULL);
-    } else if (x * per < t.queries) {
-      tc_fence_after();
-      const long long q_row = (long long)t.q0 + query;
-      if (n > 0 && *unclean) {
-        if (mine) plain_row(p, q_row, kh * p.group + head, t.k0, lim);
-      } else {
-        // through shared memory (the queries are read), so that a row leaves in whole lines
-        const float inv = 1.f / l;
-        const bool none = begin == n || lim <= 0;
-        constexpr int PIECES = DP / 8;
-        uint8_t *out = gen + x * Cfg::PANELS * 16384 + (warp & 3) * 32 * (DP * 2);
-#pragma unroll
-        for (int d = 0; d < DP; d += 32) {
-          uint32_t o[32];
-          if (begin < n) {
-            tmem_ld_x32(t_o + d, o);
-            tmem_ld_wait();
-          }
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const __nv_bfloat162 h = none ? __floats2bfloat162_rn(0.f, 0.f)
-                                            : __floats2bfloat162_rn(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
-              w[k] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-            const int piece = (d + i) / 8;
-            *reinterpret_cast<uint4 *>(out + lane * (DP * 2) + ((piece ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        }
-        __syncwarp();
-        __nv_bfloat16 *y = static_cast<__nv_bfloat16 *>(p.y) + (long long)t.q0 * p.ldy + (long long)kh * p.group * p.dim;
-#pragma unroll 4
-        for (int i = lane; i < 32 * PIECES; i += 32) {
-          const int rr = i / PIECES, piece = i % PIECES, at = (warp & 3) * 32 + rr;
-          const int qi = at / p.group, hi = at - qi * p.group, qq = x * per + qi;
-          if (qi < per && qq < t.queries && piece * 8 < p.dim)
-            *reinterpret_cast<uint4 *>(y + qq * p.ldy + hi * p.dim + piece * 8) = *reinterpret_cast<const uint4 *>(out + rr * (DP * 2) + ((piece ^ (rr & 7)) << 4));
-        }
-      }
     }
   } else {
     if constexpr (Cfg::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");   // the whole group of warps, the idle ones too
     if (warp == 4 * TILES) {
-      if (lane == 0 && n > 0) {
-        bool ok = true;
-        const int tiles = first_turn(TILES - 1) < n ? TILES : 1;
-        mbar_arrive_expect_tx(bar_q, tiles * Cfg::PANELS * 128 * p.group * per);
-        for (int x = 0; x < tiles; ++x)
-          for (int c = 0; c < Cfg::PANELS; ++c)
-            tma_load_3d(sm_q + (x * Cfg::PANELS + c) * 16384, &tm_q, bar_q, 64 * c, kh * p.group, t.q0 + x * per);
-        for (int i = 0; i < 2 * n; ++i) {   // K and V in turn
-          const uint32_t st = i % ST, ph = (i / ST) & 1;
-          const int row = t.k0 + (n - 1 - (i >> 1)) * KEYS;
-          if (!(ok = mbar_wait_relaxed(bar_empty + 8 * st, ph ^ 1u, abort_flag))) break;
-          mbar_arrive_expect_tx(bar_full + 8 * st, Cfg::TILE);
-          for (int c = 0; c < Cfg::PANELS; ++c)
-            tma_load_3d(sm_ring + st * Cfg::TILE + c * Cfg::PANEL, i & 1 ? &tm_v : &tm_k, bar_full + 8 * st, 64 * c, kh, row);
+      uint32_t slot = 0, ph = 0, index = blockIdx.x;   // ring slot of the next load, its parity; the tile at hand
+      int sent = 0, loaded = 0;                        // tiles in the mail so far; tiles whose queries were loaded
+      bool ok = true;
+      auto mail_to_all = [&](const PromptTile &t) -> bool {
+        if (!warp_wait_long(bar_read + 8 * (sent & 1), ((sent >> 1) & 1) ^ 1u, abort_flag)) return false;
+        if (lane == 0) {
+          mail[sent & 1] = t;
+          mbar_arrive(bar_mail + 8 * (sent & 1));
         }
-        if (!ok) {
-          *abort_flag = 1;
-          report(p.status, DEV_WAIT_SMEM_EMPTY);
-          const uint64_t t0 = globaltimer();   // copies in flight land before the block ends
-          while (globaltimer() - t0 < 200000ull) {}
+        __syncwarp();
+        ++sent;
+        return true;
+      };
+      for (int i = 0;; ++i) {
+        if (lane == 0) ask_for_block(answer + 16 * (i & 1), bar_next + 8 * (i & 1));
+        PromptTile t = find_tile(p, table, index / p.kv_heads);
+        if (t.queries > 0) {
+          t.kh = index % p.kv_heads;
+          if (!(ok = mail_to_all(t))) break;
+          const int n = (seen(p, t, t.queries - 1) + KEYS - 1) / KEYS;
+          if (n > 0) {
+            const int tiles = t.queries > per ? TILES : 1, qs = loaded % QS;
+            if (!(ok = warp_wait_long(bar_qe + 8 * qs, ((loaded / QS) & 1) ^ 1u, abort_flag))) break;
+            ++loaded;
+            if (lane == 0) {
+              mbar_arrive_expect_tx(bar_q + 8 * qs, tiles * Cfg::PANELS * 128 * p.group * per);
+              for (int x = 0; x < tiles; ++x)
+                for (int k = 0; k < Cfg::PANELS; ++k)
+                  tma_load_3d(sm_q + qs * Cfg::Q + (x * Cfg::PANELS + k) * 16384, &tm_q, bar_q + 8 * qs, 64 * k, t.kh * p.group, t.q0 + x * per);
+            }
+            for (int it = 0; it < 2 * n; ++it) {   // K and V in turn
+              if (!(ok = warp_wait_long(bar_empty + 8 * slot, ph ^ 1u, abort_flag))) break;
+              if (lane == 0) {
+                mbar_arrive_expect_tx(bar_full + 8 * slot, Cfg::TILE);
+                for (int k = 0; k < Cfg::PANELS; ++k)
+                  tma_load_3d(sm_ring + slot * Cfg::TILE + k * Cfg::PANEL, it & 1 ? &tm_v : &tm_k, bar_full + 8 * slot, 64 * k, t.kh,
+                              t.k0 + (n - 1 - (it >> 1)) * KEYS);
+              }
+              if (++slot == ST) slot = 0, ph ^= 1;
+            }
+            if (!ok) break;
+          }
         }
+        if (!(ok = warp_wait_long(bar_next + 8 * (i & 1), (i >> 1) & 1, abort_flag))) break;
+        const bool given = block_given(answer + 16 * (i & 1), index);
+        fence_proxy_async();   // the answer is read before the one after the next may overwrite it
+        __syncwarp();
+        if (!given) {          // no block is left; nobody asks again
+          PromptTile end{};
+          end.queries = -1;
+          ok = mail_to_all(end);
+          break;
+        }
+      }
+      if (!ok && lane == 0) {
+        *abort_flag = 1;
+        report(p.status, DEV_WAIT_SMEM_EMPTY);
+        const uint64_t t0 = globaltimer();   // copies in flight land before the block ends
+        while (globaltimer() - t0 < 200000ull) {}
       }
     } else if (warp == 4 * TILES + 1) {
       // descriptors: 128-byte swizzle, 1024 bytes between groups of 8 rows, version 1
@@ -632,77 +750,106 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | (((uint32_t)KEYS >> 3) << 17) | ((128u >> 4) << 24);
       const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
       const uint32_t leader = lane == 0;
-      const uint32_t q_lo = kmajor | uniform(sm_q >> 4), ring = uniform(sm_ring >> 4), tm = uniform(tmem);   // below 2^14: no carry into the next field
-      const int turns = (int)uniform((uint32_t)n), visible = (int)uniform((uint32_t)lim_lo);
-      int begin[TILES];
-#pragma unroll
-      for (int x = 0; x < TILES; ++x) begin[x] = (int)uniform((uint32_t)first_turn(x));
-      bool ok = true;
-      auto scores = [&](int x, int it) -> bool {
-        const uint32_t st = (uint32_t)(2 * it) % ST, ph = ((uint32_t)(2 * it) / ST) & 1;
-        if (it >= begin[x]) {
-          if (!warp_wait(bar_full + 8 * st, ph, abort_flag)) return false;
-          tc_fence_after();
-          const uint32_t k_lo = kmajor | (ring + st * (Cfg::TILE >> 4));
-#pragma unroll
-          for (int kk = 0; kk < DP / 16; ++kk)
-            umma_ss(leader, tm + Cfg::S_COL + x * Cfg::STEP, desc_hi | (q_lo + (x * Cfg::PANELS + (kk >> 2)) * 1024 + (kk & 3) * 2),
-                    desc_hi | (k_lo + (kk >> 2) * (Cfg::PANEL >> 4) + (kk & 3) * 2), idesc_s, kk != 0);
-          commit_if(leader, bar_s + 8 * x);
-        }
-        if (x == TILES - 1) commit_if(leader, bar_empty + 8 * st);   // both tiles' products with these keys are on their way
-        return true;
+      const uint32_t q_all = kmajor | uniform(sm_q >> 4), ring = uniform(sm_ring >> 4), tm = uniform(tmem);   // below 2^14: no carry into the next field
+      uint32_t ks = 0, kph = 0, vs = 1 % ST, vph = 0;   // ring slots of the next keys and values, with their parities
+      auto step = [](uint32_t &slot, uint32_t &ph) {
+        slot += 2;
+        if (slot >= ST) slot -= ST, ph ^= 1;
       };
-      if (turns > 0) ok = warp_wait(bar_q, 0, abort_flag);
+      uint32_t scored[TILES] = {}, weighed[TILES] = {}, results[TILES] = {};   // products so far, tile of rows by tile
+      int loaded = 0;
+      bool ok = true;
+      PromptTile t;
+      for (int i = 0; ok && (ok = receive(i, t)) && t.queries > 0; ++i) {
+        const int lim_lo = seen(p, t, 0), lim_hi = seen(p, t, t.queries - 1);
+        const int n = (int)uniform((lim_hi + KEYS - 1) / KEYS), visible = (int)uniform(lim_lo);
+        if (n == 0) continue;
+        int begin[TILES];
 #pragma unroll
-      for (int x = 0; x < TILES; ++x)
-        if (turns > 0 && ok) ok = scores(x, 0);
-      for (int it = 0; it < turns && ok; ++it) {
-        const int base = (turns - 1 - it) * KEYS;
-        const uint32_t st = (uint32_t)(2 * it + 1) % ST, ph = ((uint32_t)(2 * it + 1) / ST) & 1;
-        if (Cfg::EARLY && it + 1 < turns && !(ok = warp_wait(bar_se, it & 1, abort_flag) && scores(0, it + 1))) break;
-        if (!(ok = warp_wait(bar_full + 8 * st, ph, abort_flag))) break;
-        if (base + KEYS > visible) {
-          // Values past the last key that anybody here sees belong to others and may hold anything: zeros in their place, since
-          // the tensor cores multiply every value by every row's weight and 0 * NaN is NaN.  Values on the diagonal are hidden
-          // from some rows only: if one is not finite, the rows are summed up the plain way at the end.
-          uint8_t *v = gen + Cfg::Q + st * Cfg::TILE;
-          constexpr int PIECES = 8 * Cfg::PANELS;   // 16-byte pieces of a key's values
-          const int none = max(0, min(KEYS, lim_hi - base)), some = max(0, min(none, lim_lo - base));
-          for (int i = none * PIECES + lane; i < KEYS * PIECES; i += 32) {
-            const int key = i / PIECES, piece = i % PIECES;
-            *reinterpret_cast<uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
-          }
-          bool bad = false;
-          for (int i = some * PIECES + lane; i < none * PIECES; i += 32) {
-            const int key = i / PIECES, piece = i % PIECES;
-            const uint4 w = *reinterpret_cast<const uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16);
-            for (uint32_t u : {w.x, w.y, w.z, w.w}) bad |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
-          }
-          if (bad) *unclean = 1;
-          fence_proxy_async();
-          __syncwarp();
-        }
-        const uint32_t v_lo = mnmajor | (ring + st * (Cfg::TILE >> 4));
-#pragma unroll
-        for (int x = 0; x < TILES; ++x) {
+        for (int x = 0; x < TILES; ++x) begin[x] = (int)uniform(first_turn(t, n, x));
+        const uint32_t qs = loaded % QS, q_lo = q_all + qs * (Cfg::Q >> 4);
+        auto scores = [&](int x, int it) -> bool {
           if (it >= begin[x]) {
-            if (!(ok = warp_wait(bar_p + 8 * x, (it - begin[x]) & 1, abort_flag))) break;
+            if (Cfg::EARLY && scored[x] > 0 && !warp_wait(bar_se + 8 * x, (scored[x] - 1) & 1, abort_flag)) return false;
+            if (!warp_wait(bar_full + 8 * ks, kph, abort_flag)) return false;
             tc_fence_after();
-            const uint32_t more = it != begin[x];
+            const uint32_t k_lo = kmajor | (ring + ks * (Cfg::TILE >> 4));
 #pragma unroll
-            for (int kk = 0; kk < KEYS / 16; ++kk)   // 16 keys: 8 columns of P, 16 rows of V
-              umma_ts(leader, tm + Cfg::O_COL + x * Cfg::STEP, tm + Cfg::P_COL + x * Cfg::STEP + 8 * kk, desc_hi | (v_lo + 128 * kk), idesc_o,
-                      kk != 0 ? 1u : more);
+            for (int kk = 0; kk < DP / 16; ++kk)
+              umma_ss(leader, tm + Cfg::S_COL + x * Cfg::STEP, desc_hi | (q_lo + (x * Cfg::PANELS + (kk >> 2)) * 1024 + (kk & 3) * 2),
+                      desc_hi | (k_lo + (kk >> 2) * (Cfg::PANEL >> 4) + (kk & 3) * 2), idesc_s, kk != 0);
+            commit_if(leader, bar_s + 8 * x);
+            ++scored[x];
           }
-          if (x == TILES - 1) commit_if(leader, bar_empty + 8 * st);
-          if (it + 1 == turns && begin[x] < turns) {
-            commit_if(leader, bar_o + 8 * x);
-            if (lane == 0) mbar_arrive(bar_o + 8 * x);
+          if (x == TILES - 1) {   // both tiles' products with these keys are on their way
+            commit_if(leader, bar_empty + 8 * ks);
+            step(ks, kph);
+            if (it + 1 == n) commit_if(leader, bar_qe + 8 * qs);
           }
-          // Without columns of their own the weights lie where the next scores go.  Both products are this thread's, and the
-          // tensor cores take them in order.
-          if (!Cfg::EARLY && it + 1 < turns && !(ok = scores(x, it + 1))) break;
+          return true;
+        };
+        if (!(ok = warp_wait(bar_q + 8 * qs, (loaded / QS) & 1, abort_flag))) break;
+        ++loaded;
+#pragma unroll
+        for (int x = 0; x < TILES; ++x)
+          if (ok) ok = scores(x, 0);
+        for (int it = 0; it < n && ok; ++it) {
+          const int base = (n - 1 - it) * KEYS;
+          if (Cfg::EARLY && it + 1 < n && !(ok = scores(0, it + 1))) break;
+          if (!(ok = warp_wait(bar_full + 8 * vs, vph, abort_flag))) break;
+          if (base + KEYS > visible) {
+            // Values past the last key that anybody here sees belong to others and may hold anything: zeros in their place, since
+            // the tensor cores multiply every value by every row's weight and 0 * NaN is NaN.  Values on the diagonal are hidden
+            // from some rows only: if one is not finite, the rows are summed up the plain way at the end.
+            uint8_t *v = gen + QS * Cfg::Q + vs * Cfg::TILE;
+            constexpr int PIECES = 8 * Cfg::PANELS;   // 16-byte pieces of a key's values
+            const int none = max(0, min(KEYS, lim_hi - base)), some = max(0, min(none, lim_lo - base));
+            for (int k = none * PIECES + lane; k < KEYS * PIECES; k += 32) {
+              const int key = k / PIECES, piece = k % PIECES;
+              *reinterpret_cast<uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            bool bad = false;
+            for (int k = some * PIECES + lane; k < none * PIECES; k += 32) {
+              const int key = k / PIECES, piece = k % PIECES;
+              const uint4 w = *reinterpret_cast<const uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16);
+              for (uint32_t u : {w.x, w.y, w.z, w.w}) bad |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
+            }
+            if (bad) unclean[i & 3] = i + 1;   // this warp is at most two tiles ahead: the mail has two places
+            fence_proxy_async();
+            __syncwarp();
+          }
+          const uint32_t v_lo = mnmajor | (ring + vs * (Cfg::TILE >> 4));
+#pragma unroll
+          for (int x = 0; x < TILES; ++x) {
+            if (it >= begin[x]) {
+              if (it == begin[x] && results[x] > 0 && !(ok = warp_wait(bar_oe + 8 * x, (results[x] - 1) & 1, abort_flag))) break;
+              const uint32_t more = it != begin[x];
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                if (!(ok = warp_wait(bar_p + 16 * x + 8 * half, weighed[x] & 1, abort_flag))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int kk = half * KEYS / 32; kk < (half + 1) * KEYS / 32; ++kk)   // 16 keys: 8 columns of P, 16 rows of V
+                  umma_ts(leader, tm + Cfg::O_COL + x * Cfg::STEP, tm + Cfg::P_COL + x * Cfg::STEP + 8 * kk, desc_hi | (v_lo + 128 * kk), idesc_o,
+                          kk != 0 ? 1u : more);
+              }
+              if (!ok) break;
+              ++weighed[x];
+              if (Cfg::EARLY) commit_if(leader, bar_pv + 8 * x);
+            }
+            if (x == TILES - 1) {
+              commit_if(leader, bar_empty + 8 * vs);
+              step(vs, vph);
+            }
+            if (it + 1 == n && begin[x] < n) {
+              commit_if(leader, bar_o + 8 * x);
+              if (lane == 0) mbar_arrive(bar_o + 8 * x);
+              ++results[x];
+            }
+            // Without columns of their own the weights lie where the next scores go.  Both products are this thread's, and the
+            // tensor cores take them in order.
+            if (!Cfg::EARLY && it + 1 < n && !(ok = scores(x, it + 1))) break;
+          }
         }
       }
       if (!ok && lane == 0) {
