@@ -198,6 +198,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
+constexpr float MARGIN = 16.f;   // see prompt_umma_kernel
 // The issuing warp stays together and one lane's predicate does the rest: the operands are then the same in every lane, which
 // lets the compiler keep them in uniform registers.  With a branch to one lane around the products every operand was moved there
 // one by one, and issuing a tile's 16 products took longer than computing them.
@@ -269,7 +270,7 @@ struct UmmaSize : UmmaCfg<DP> {
   static constexpr int TILE = C::KEYS * DP * 2;             // keys or values
   static constexpr int PANEL = C::KEYS * 128;
   // Warps of rows; then TMA, MMA.  Where a thread holds a row of 128 scores, 168 registers (12 warps' share) make it spill: the block
-  // is launched with a whole third group of warps, which hands registers over, 384 x 168 = 256 x 216 + 128 x 72.
+  // is launched with a whole third group of warps, which hands registers over, 384 x 168 = 256 x 200 + 128 x 104.
   static constexpr bool MOVE = C::TILES == 2;
   static constexpr int THREADS = C::TILES * 128 + (MOVE ? 128 : 64);
   static constexpr int CONTROL = 512 + 64 + 64 + 4 * (RUNS + 1);   // barriers, mail, answers, table of tiles
@@ -331,10 +332,9 @@ __device__ __noinline__ void plain_row(const PromptParams &p, long long q_row, i
 //   a warp           finds the tile, leaves it in the mail for the others, asks for the next; lane 0 loads by TMA: the queries once, then
 //                    per tile of keys K and V, from the last to the first, into a ring -- of the next tile while this one is computed
 //   a warp           MMA: S = Q K^T (operands in shared memory), O += P V (P in tensor memory, V MN-major in shared memory)
-//   4 warps a tile   a thread per row: maximum, exponentials, row sum; P as bf16 back to tensor memory, in two halves, the first of which
-//                    is multiplied while the second is computed
-// The reference maximum of a row moves only when a tile's maximum is 2^8 above it (weights stay below 2^8, exact in effect
-// since numerator and denominator use the same); then O is rescaled in tensor memory, which after the first tiles is rare.
+//   4 warps a tile   a thread per row: maximum, exponentials, row sum; P as bf16 back to tensor memory
+// The reference maximum of a row moves only when a tile's maximum is 2^16 above it (fp32 and bf16 keep their relative precision up
+// there, and numerator and denominator use the same); then O is rescaled in tensor memory, which is rare.
 // Only tiles that the sequence's end or the diagonal cross pay for masks.  Every wait has a limit.
 template <int DP>
 __global__ void __launch_bounds__(UmmaSize<DP>::THREADS, UmmaSize<DP>::BLOCKS)
@@ -356,8 +356,8 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const uint32_t bar_empty = bar_full + 8 * ST;      // [ST] the products that read them are complete
   const uint32_t bar_s = bar_empty + 8 * ST;         // [TILES] scores complete in tensor memory
   const uint32_t bar_se = bar_s + 8 * TILES;         // [TILES] scores read (EARLY)
-  const uint32_t bar_p = bar_se + 8 * TILES;         // [TILES][2] half of the weights written to tensor memory
-  const uint32_t bar_pv = bar_p + 16 * TILES;        // [TILES] product with the values complete (EARLY)
+  const uint32_t bar_p = bar_se + 8 * TILES;         // [TILES] weights written to tensor memory
+  const uint32_t bar_pv = bar_p + 8 * TILES;        // [TILES] product with the values complete (EARLY)
   const uint32_t bar_o = bar_pv + 8 * TILES;         // [TILES] result complete
   const uint32_t bar_oe = bar_o + 8 * TILES;         // [TILES] result read
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(tail + 448);
@@ -386,8 +386,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     for (int x = 0; x < TILES; ++x) {
       mbar_init(bar_s + 8 * x, 1);
       mbar_init(bar_se + 8 * x, 4);
-      mbar_init(bar_p + 16 * x, 4);
-      mbar_init(bar_p + 16 * x + 8, 4);
+      mbar_init(bar_p + 8 * x, 4);
       mbar_init(bar_pv + 8 * x, 1);
       mbar_init(bar_o + 8 * x, 2);   // the product, and the issuer's word on `unclean`
       mbar_init(bar_oe + 8 * x, 4);
@@ -424,7 +423,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   };
 
   if (warp < 4 * TILES) {
-    if constexpr (Cfg::MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (Cfg::MOVE) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int x = warp >> 2;                      // tile of rows
     const int row = (warp & 3) * 32 + lane;
     const int in_tile = row / p.group, head = row - in_tile * p.group, query = x * per + in_tile;
@@ -450,7 +449,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           m = top;
           return;
         }
-        const bool up = (top - m) * c > 8.f;
+        const bool up = (top - m) * c > MARGIN;
         if (!__any_sync(0xffffffffu, up)) return;
         const float f = up ? ex2((m - top) * c) : 1.f;
         if (up) m = top;
@@ -465,11 +464,11 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           tmem_st_x16(t_o + d, o);
         }
       };
-      auto hand_over = [&](int half) {   // half of P is in tensor memory
+      auto hand_over = [&]() {   // P is in tensor memory
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p + 16 * x + 8 * half);
+        if (lane == 0) mbar_arrive(bar_p + 8 * x);
       };
       for (int it = begin; it < n; ++it, ++turns) {
         const int base = (n - 1 - it) * KEYS;
@@ -511,27 +510,22 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           bool careful = masked || first;
           if (!careful) {
             // The weights by the reference maximum that is there, without waiting for this tile's own; that one is found beside
-            // the first half and, if it is more than 2^8 above (or a score is NaN or +inf), the tile is done over.
+            // them and, if it is more than 2^16 above (or a score is NaN or +inf), the tile is done over.
             const float off = -m * c;
             float2 sum = make_float2(0.f, 0.f);
             float x0 = s[0], x1 = s[1];
 #pragma unroll
-            for (int k = 0; k < KEYS / 2; k += 32) {
+            for (int k = 0; k < KEYS; k += 32) {
               weigh(k, make_float2(off, off), sum);
 #pragma unroll
-              for (int e = 2 * k; e < 2 * k + 64; e += 4) {
+              for (int e = k; e < k + 32; e += 4) {
                 x0 = max3_nan(x0, s[e], s[e + 1]);
                 x1 = max3_nan(x1, s[e + 2], s[e + 3]);
               }
             }
             const float top = max3_nan(x0, x1, x1);
-            careful = __any_sync(0xffffffffu, mine && !((top - m) * c <= 8.f));
-            if (!careful) {
-              hand_over(0);
-#pragma unroll
-              for (int k = KEYS / 2; k < KEYS; k += 32) weigh(k, make_float2(off, off), sum);
-              l += sum.x + sum.y;
-            }
+            careful = __any_sync(0xffffffffu, mine && !((top - m) * c <= MARGIN));
+            if (!careful) l += sum.x + sum.y;
           }
           if (careful) {
             tmem_st_wait();   // what the first attempt wrote is written again
@@ -550,9 +544,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
             for (int k = 0; k < KEYS; k += 32) weigh(k, make_float2(off, off), sum);
             l += sum.x + sum.y;
-            hand_over(0);
           }
-          hand_over(1);
         } else {
           // twice from tensor memory, 32 columns at a time: once for the maximum, once for the weights
           uint32_t r[32], other[32];
@@ -623,11 +615,10 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               if (lane == 0) mbar_arrive(bar_se + 8 * x);
             }
             weigh(other, k + 32);
-            if (k + 64 == KEYS / 2) hand_over(0);
           }
           l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-          hand_over(1);
         }
+        hand_over();
       }
       if (!ok) break;
       const long long q_row = (long long)t.q0 + query;
@@ -681,7 +672,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       report(p.status, DEV_WAIT_TMEM_FULL);
     }
   } else {
-    if constexpr (Cfg::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");   // the whole group of warps, the idle ones too
+    if constexpr (Cfg::MOVE) asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");   // the whole group of warps, the idle ones too
     if (warp == 4 * TILES) {
       uint32_t slot = 0, ph = 0, index = blockIdx.x;   // ring slot of the next load, its parity; the tile at hand
       int sent = 0, loaded = 0;                        // tiles in the mail so far; tiles whose queries were loaded
@@ -824,16 +815,12 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             if (it >= begin[x]) {
               if (it == begin[x] && results[x] > 0 && !(ok = warp_wait(bar_oe + 8 * x, (results[x] - 1) & 1, abort_flag))) break;
               const uint32_t more = it != begin[x];
+              if (!(ok = warp_wait(bar_p + 8 * x, weighed[x] & 1, abort_flag))) break;
+              tc_fence_after();
 #pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                if (!(ok = warp_wait(bar_p + 16 * x + 8 * half, weighed[x] & 1, abort_flag))) break;
-                tc_fence_after();
-#pragma unroll
-                for (int kk = half * KEYS / 32; kk < (half + 1) * KEYS / 32; ++kk)   // 16 keys: 8 columns of P, 16 rows of V
-                  umma_ts(leader, tm + Cfg::O_COL + x * Cfg::STEP, tm + Cfg::P_COL + x * Cfg::STEP + 8 * kk, desc_hi | (v_lo + 128 * kk), idesc_o,
-                          kk != 0 ? 1u : more);
-              }
-              if (!ok) break;
+              for (int kk = 0; kk < KEYS / 16; ++kk)   // 16 keys: 8 columns of P, 16 rows of V
+                umma_ts(leader, tm + Cfg::O_COL + x * Cfg::STEP, tm + Cfg::P_COL + x * Cfg::STEP + 8 * kk, desc_hi | (v_lo + 128 * kk), idesc_o,
+                        kk != 0 ? 1u : more);
               ++weighed[x];
               if (Cfg::EARLY) commit_if(leader, bar_pv + 8 * x);
             }
