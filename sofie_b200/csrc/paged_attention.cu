@@ -36,19 +36,6 @@ struct PagedAttnParams {
   float *part_o;              // [grid * 2][16][DP]
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void *src, bool there) {   // zeros where there is nothing
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -307,7 +294,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_mma_kernel(const __grid_cons
       const bool up0 = x0 > m0 + 8.f, up1 = x1 > m1 + 8.f;
       if (__any_sync(0xffffffffu, up0 || up1)) {
         const float n0 = up0 ? x0 : m0, n1 = up1 ? x1 : m1;
-        const float f0 = up0 ? exp2_fast(m0 - n0) : 1.f, f1 = up1 ? exp2_fast(m1 - n1) : 1.f;
+        const float f0 = up0 ? ex2(m0 - n0) : 1.f, f1 = up1 ? ex2(m1 - n1) : 1.f;
         m0 = n0;
         m1 = n1;
         l0 *= f0;
@@ -324,7 +311,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_mma_kernel(const __grid_cons
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           const float mm = half ? m1 : m0;
-          const float e0 = exp2_fast(s[t][2 * half] - mm), e1 = exp2_fast(s[t][2 * half + 1] - mm);
+          const float e0 = ex2(s[t][2 * half] - mm), e1 = ex2(s[t][2 * half + 1] - mm);
           if (half) l1 += e0 + e1;
           else l0 += e0 + e1;
           const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
@@ -367,10 +354,10 @@ __global__ void __launch_bounds__(PA_THREADS) paged_mma_kernel(const __grid_cons
     const float B0 = M0 == -INFINITY ? 0.f : M0, B1 = M1 == -INFINITY ? 0.f : M1;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      L0 += merge_l[w * PA_ROWS + r0] * exp2_fast(merge_m[w * PA_ROWS + r0] - B0);
-      L1 += merge_l[w * PA_ROWS + r1] * exp2_fast(merge_m[w * PA_ROWS + r1] - B1);
+      L0 += merge_l[w * PA_ROWS + r0] * ex2(merge_m[w * PA_ROWS + r0] - B0);
+      L1 += merge_l[w * PA_ROWS + r1] * ex2(merge_m[w * PA_ROWS + r1] - B1);
     }
-    const float f0 = exp2_fast(m0 - B0), f1 = exp2_fast(m1 - B1);
+    const float f0 = ex2(m0 - B0), f1 = ex2(m1 - B1);
 #pragma unroll
     for (int i = 0; i < DP / 8; ++i) {
       o[i][0] *= f0; o[i][1] *= f0;
@@ -714,7 +701,7 @@ __global__ void paged_join_kernel(const __grid_constant__ PagedAttnParams p, int
 #pragma unroll 4
   for (int i = 0; i < parts; ++i) {
     const long long s = slot(i);
-    const float f = exp2_fast(p.part_m[s] - base);
+    const float f = ex2(p.part_m[s] - base);
     L += p.part_l[s] * f;
     o += p.part_o[s * dp + d] * f;
   }

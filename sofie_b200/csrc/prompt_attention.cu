@@ -119,59 +119,177 @@ __device__ __forceinline__ int seen(const PromptParams &p, const PromptTile &t, 
   return p.causal ? min(t.k_len, max(0, t.past + i)) : t.k_len;
 }
 
-// ---- fp32 (and the first form of every type): one warp per (query, head), lane l holds dimensions l, l + 32, ... ----------------
-// Softmax in one pass with a running maximum: a larger maximum scales the sum and the weighted values so far.
-template <class T>
-__global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptParams p) {
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const long long t = w / p.heads;
-  const int h = (int)(w % p.heads);
-  if (t >= p.q_rows) return;
-  const int b = packed_find(p.cu_q, p.batch, (int)t);
-  if (b < 0) return;
-  int q0, q1, k0, k1;
-  bool bad = false;
-  packed_range(p.cu_q, b, p.q_rows, &q0, &q1, &bad);
-  packed_range(p.cu_k, b, p.k_rows, &k0, &k1, &bad);
-  if (bad) {
-    report(p.status, DEV_BAD_INDEX);
-    return;
-  }
-  int n = k1 - k0;
-  if (p.causal) n = min(n, max(0, (int)(t - q0) + 1 + n - (q1 - q0)));
-  const int kh = h / (p.heads / p.kv_heads);
-  const T *q = static_cast<const T *>(p.q) + t * p.ldq + h * p.dim;
-  float qr[8], acc[8];
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    qr[i] = d < p.dim ? to_f32(q[d]) * p.scale_log2e : 0.f;
-    acc[i] = 0.f;
-  }
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < n; ++j) {
-    const T *k = static_cast<const T *>(p.k) + (k0 + j) * p.ldk + kh * p.dim;
-    const T *v = static_cast<const T *>(p.v) + (k0 + j) * p.ldv + kh * p.dim;
-    float s = 0.f;
-    for (int i = 0; i < 8; ++i) {
-      const int d = lane + 32 * i;
-      if (d < p.dim) s = fmaf(qr[i], to_f32(k[d]), s);
+// ---- fp32 on the CUDA cores --------------------------------------------------------------------------------------------------------
+// A block of four warps computes 32 rows against tiles of 64 keys.  A thread has 4 rows x 4 keys of the scores and 4 rows x DP / 16
+// dimensions of the result, so that a 16-byte read from shared memory feeds 16 FMAs and the FMA pipes are what bounds it.  The next
+// keys arrive while this tile's values are weighed, the next values while the next scores are computed (cp.async, one place each).
+constexpr int PF_ROWS = 32, PF_KEYS = 64, PF_THREADS = 128;
+template <int DP>
+struct FmaCfg {
+  static constexpr int Q = PF_ROWS * DP * 4, TILE = PF_KEYS * DP * 4, P = PF_KEYS * PF_ROWS * 4;
+  static constexpr int SMEM = Q + 2 * TILE + P + 4 * (RUNS + 1);
+};
+
+template <int DP>
+__global__ void __launch_bounds__(PF_THREADS) prompt_fma_kernel(const __grid_constant__ PromptParams p, int parts) {
+  using Cfg = FmaCfg<DP>;
+  constexpr int CH = DP / 4, PIECES = DP / 64;   // 16-byte pieces of a row; of the result per thread and row
+  extern __shared__ __align__(128) uint8_t smem[];
+  float4 *sq = reinterpret_cast<float4 *>(smem), *sk = sq + Cfg::Q / 16, *sv = sk + Cfg::TILE / 16, *sp = sv + Cfg::TILE / 16;
+  int *table = reinterpret_cast<int *>(smem + Cfg::Q + 2 * Cfg::TILE + Cfg::P);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  count_tiles(p, table);
+  const int work = blockIdx.x / parts, part = blockIdx.x % parts, kh = work % p.kv_heads;   // a group of more than 32 heads is several parts
+  const PromptTile t = find_tile(p, table, work / p.kv_heads);
+  if (t.queries == 0) return;
+  const int head0 = part * PF_ROWS, heads = min(PF_ROWS, p.group - head0);   // heads of the group in this block
+  const int lim_lo = seen(p, t, 0), lim_hi = seen(p, t, t.queries - 1);
+  const int n = (lim_hi + PF_KEYS - 1) / PF_KEYS;
+  const float *q = static_cast<const float *>(p.q) + t.q0 * p.ldq + (long long)(kh * p.group + head0) * p.dim;
+  const float *k = static_cast<const float *>(p.k) + t.k0 * p.ldk + (long long)kh * p.dim;
+  const float *v = static_cast<const float *>(p.v) + t.k0 * p.ldv + (long long)kh * p.dim;
+  const uint32_t a_q = smem_u32(sq), a_k = smem_u32(sk), a_v = smem_u32(sv);
+
+  auto load_tile = [&](uint32_t dst, const float *src, long long pitch, int base, bool swizzle) {
+#pragma unroll 4
+    for (int i = tid; i < PF_KEYS * CH; i += PF_THREADS) {
+      const int r = i / CH, c = i % CH;
+      const bool there = base + r < lim_hi && c * 4 < p.dim;
+      cp_async_16(dst + (r * CH + (swizzle ? c ^ (r & 7) : c)) * 16, src + (there ? (base + r) * pitch + c * 4 : 0), there);
     }
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const float m1 = fmaxf(m, s), base = m1 == -INFINITY ? 0.f : m1;
-    const float f = exp2f(m - base), e = exp2f(s - base);
-    m = m1;
-    l = l * f + e;
-    for (int i = 0; i < 8; ++i) {
-      const int d = lane + 32 * i;
-      if (d < p.dim) acc[i] = acc[i] * f + e * to_f32(v[d]);
-    }
+  };
+  for (int i = tid; i < PF_ROWS * CH; i += PF_THREADS) {
+    const int r = i / CH, c = i % CH, query = r / heads, h = r - query * heads;
+    const bool there = query < t.queries && c * 4 < p.dim;
+    cp_async_16(a_q + i * 16, q + (there ? query * p.ldq + (long long)h * p.dim + c * 4 : 0), there);
   }
-  T *y = static_cast<T *>(p.y) + t * p.ldy + h * p.dim;
-  const float inv = n > 0 ? 1.f / l : 0.f;
-  for (int i = 0; i < 8; ++i) {
-    const int d = lane + 32 * i;
-    if (d < p.dim) from_f32(y + d, acc[i] * inv);
+  if (n > 0) load_tile(a_k, k, p.ldk, (n - 1) * PF_KEYS, true);
+  cp_async_commit();
+  if (n > 0) load_tile(a_v, v, p.ldv, (n - 1) * PF_KEYS, false);
+  cp_async_commit();
+
+  const int rg = warp * 2 + (lane >> 4), g = lane & 15;   // rows 4 rg .. 4 rg + 3; keys g + 16 j; pieces g + 16 j of the result
+  int lim[4];
+  float m[4], l[4];
+  float4 acc[4][PIECES];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int query = (4 * rg + r) / heads;
+    lim[r] = query < t.queries ? seen(p, t, query) : 0;
+    m[r] = -INFINITY;   // in units of log2; -inf: no key yet
+    l[r] = 0.f;         // this thread's keys only
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) acc[r][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+
+  for (int it = n - 1; it >= 0; --it) {
+    const int base = it * PF_KEYS;
+    const bool masked = base + PF_KEYS > lim_lo;
+    cp_async_wait<1>();   // the keys
+    __syncthreads();
+    float s[4][4] = {};
+#pragma unroll 2
+    for (int c = 0; c < CH; ++c) {
+      float4 a[4], b[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) a[r] = sq[(4 * rg + r) * CH + c];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = sk[(g + 16 * j) * CH + (c ^ (g & 7))];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[r][j] = fmaf(a[r].x, b[j].x, fmaf(a[r].y, b[j].y, fmaf(a[r].z, b[j].z, fmaf(a[r].w, b[j].w, s[r][j]))));
+    }
+    __syncthreads();   // the keys are read
+    if (it > 0) load_tile(a_k, k, p.ldk, base - PF_KEYS, true);
+    cp_async_commit();
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[r][j] = base + g + 16 * j < lim[r] ? s[r][j] * p.scale_log2e : -INFINITY;
+        top = fmaxf(top, s[r][j]);
+      }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (base < lim[r]) top = fmaxf(top, -3.0e38f);   // a key is there: the maximum is a number
+      if (top > m[r]) {
+        const float f = ex2(m[r] - top);
+        m[r] = top;
+        l[r] *= f;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) { acc[r][j].x *= f; acc[r][j].y *= f; acc[r][j].z *= f; acc[r][j].w *= f; }
+      }
+      const float off = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[r][j] = ex2(s[r][j] - off);
+        l[r] += s[r][j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int key = g + 16 * j;
+      sp[key * (PF_ROWS / 4) + (rg ^ (key & 7))] = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
+    }
+    cp_async_wait<1>();   // the values
+    __syncthreads();
+    if (!masked) {
+#pragma unroll 4
+      for (int key = 0; key < PF_KEYS; ++key) {
+        const float4 w = sp[key * (PF_ROWS / 4) + (rg ^ (key & 7))];
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const float4 x = sv[key * CH + g + 16 * j];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float e = r == 0 ? w.x : r == 1 ? w.y : r == 2 ? w.z : w.w;
+            acc[r][j].x = fmaf(e, x.x, acc[r][j].x);
+            acc[r][j].y = fmaf(e, x.y, acc[r][j].y);
+            acc[r][j].z = fmaf(e, x.z, acc[r][j].z);
+            acc[r][j].w = fmaf(e, x.w, acc[r][j].w);
+          }
+        }
+      }
+    } else {   // a hidden value may be NaN or infinite: it is left out, not multiplied by 0
+      for (int key = 0; key < PF_KEYS; ++key) {
+        const float4 w = sp[key * (PF_ROWS / 4) + (rg ^ (key & 7))];
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+          const float4 x = sv[key * CH + g + 16 * j];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float e = r == 0 ? w.x : r == 1 ? w.y : r == 2 ? w.z : w.w;
+            if (base + key < lim[r]) {
+              acc[r][j].x = fmaf(e, x.x, acc[r][j].x);
+              acc[r][j].y = fmaf(e, x.y, acc[r][j].y);
+              acc[r][j].z = fmaf(e, x.z, acc[r][j].z);
+              acc[r][j].w = fmaf(e, x.w, acc[r][j].w);
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();   // values and weights are read
+    if (it > 0) load_tile(a_v, v, p.ldv, base - PF_KEYS, false);
+    cp_async_commit();
+  }
+  cp_async_wait<0>();
+
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], o);
+    const int at = 4 * rg + r, query = at / heads, h = at - query * heads;
+    if (query >= t.queries) continue;
+    const float inv = m[r] == -INFINITY ? 0.f : 1.f / l[r];
+    float *y = static_cast<float *>(p.y) + (t.q0 + query) * p.ldy + (long long)(kh * p.group + head0 + h) * p.dim;
+#pragma unroll
+    for (int j = 0; j < PIECES; ++j) {
+      const int d = (g + 16 * j) * 4;
+      if (d < p.dim) *reinterpret_cast<float4 *>(y + d) = make_float4(acc[r][j].x * inv, acc[r][j].y * inv, acc[r][j].z * inv, acc[r][j].w * inv);
+    }
   }
 }
 
@@ -187,11 +305,6 @@ __device__ __forceinline__ bool warp_wait_long(uint32_t bar, uint32_t parity, vo
 }
 
 // ---- bf16 on the tensor cores --------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // max(a, b, c), NaN if one of them is
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float y;
@@ -901,6 +1014,20 @@ static int launch_umma(sofie_b200_ctx *ctx, PromptParams p) {
   return 0;
 }
 
+template <int DP>
+static int launch_fma(sofie_b200_ctx *ctx, PromptParams p) {
+  const int parts = (p.group + PF_ROWS - 1) / PF_ROWS;
+  p.tokens = parts > 1 ? 1 : PF_ROWS / p.group;
+  const long long grid = (p.q_rows / p.tokens + p.batch) * p.kv_heads * parts;
+  if (grid > 0x7fffffffLL) return fail(SOFIE_B200_ERR_TOO_LARGE, "prompt_attention_enqueue: %lld queries of %d heads", p.q_rows, p.heads);
+  if (!p.k_rows) p.k = p.v = p.q;   // nothing is read, but the address a copy of no bytes is given should exist
+  SB_CUDA(cudaFuncSetAttribute(prompt_fma_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, FmaCfg<DP>::SMEM));   // per device
+  prompt_fma_kernel<DP><<<(unsigned)grid, PF_THREADS, FmaCfg<DP>::SMEM, ctx->stream>>>(p, parts);
+  SB_CUDA(cudaGetLastError());
+  ctx->launches++;
+  return 0;
+}
+
 }  // namespace sb200
 
 using namespace sb200;
@@ -946,7 +1073,7 @@ int sofie_b200_prompt_attention_plan_destroy(sofie_b200_prompt_attention_plan *p
 }
 
 const char *sofie_b200_prompt_attention_plan_kernel(const sofie_b200_prompt_attention_plan *plan) {
-  return !plan ? "" : plan->d.dtype == SOFIE_B200_F32 ? "rows" : "umma";
+  return !plan ? "" : plan->d.dtype == SOFIE_B200_F32 ? "fma" : "umma";
 }
 
 int sofie_b200_prompt_attention_enqueue(sofie_b200_prompt_attention_plan *plan, const void *q, const void *k, const void *v, void *y,
@@ -977,12 +1104,9 @@ int sofie_b200_prompt_attention_enqueue(sofie_b200_prompt_attention_plan *plan, 
     if (d.head_dim <= 128) return launch_umma<128>(ctx, p);
     return launch_umma<256>(ctx, p);
   }
-  const int64_t blocks = (q_tokens * d.heads + 3) / 4;
-  if (blocks > 0x7fffffffLL) return fail(SOFIE_B200_ERR_TOO_LARGE, "prompt_attention_enqueue: %lld queries of %d heads", (long long)q_tokens, d.heads);
-  prompt_rows_kernel<float><<<(unsigned)blocks, 128, 0, ctx->stream>>>(p);
-  SB_CUDA(cudaGetLastError());
-  ctx->launches++;
-  return 0;
+  if (d.head_dim <= 64) return launch_fma<64>(ctx, p);
+  if (d.head_dim <= 128) return launch_fma<128>(ctx, p);
+  return launch_fma<256>(ctx, p);
 }
 
 }  // extern "C"
