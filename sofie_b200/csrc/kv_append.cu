@@ -73,70 +73,180 @@ struct AppendParams {
   int *status;
 };
 
-// One block per token.  An element pair (first, second) that turns together is one thread's work, so q_out may be q.
-template <class T>
+// Position of token t and the element offset of its place in the cache (negative: no place, the token is left out), found by a warp:
+// 32 offsets of cu_seqlens at a time, so two rounds of loads for a thousand sequences.
+__device__ __forceinline__ long long find_place(const AppendParams &p, int t, int *pos_out) {
+  const int lane = threadIdx.x & 31;
+  int b = t;
+  if (p.cu) {
+    int lo = 0, hi = p.kv.batch;
+    while (hi - lo > 1) {
+      const int at = search_probe(lo, hi, lane);
+      const uint32_t below = __ballot_sync(0xffffffffu, at < hi && p.cu[at] <= t);
+      search_narrow(lo, hi, below ? 31 - __clz(below) : 0);
+    }
+    b = p.cu[lo] <= t && t < p.cu[lo + 1] ? lo : -1;
+  }
+  if (b < 0) return -1;
+  const int len = p.kv.lens[b];
+  int pos = len - 1;
+  if (p.cu) {
+    int begin, end;
+    bool bad = false;
+    packed_range(p.cu, b, p.tokens, &begin, &end, &bad);
+    pos = bad ? -1 : len - (end - t);
+  }
+  long long row = -1;
+  if (pos >= 0 && (p.half == 0 || pos < p.max_position)) row = paged_row(p.kv, b, pos);
+  if (row < 0 && !(p.cu == nullptr && len == 0) && lane == 0) report(p.status, DEV_BAD_INDEX);
+  *pos_out = pos;
+  return row;
+}
+
+// A piece of V elements as they lie in memory (V * sizeof(T) = 16, 8, 4 or 2 bytes).
+template <class T, int V>
+struct alignas(sizeof(T) * V) Piece {
+  T x[V];
+};
+
+// One block per token, a thread per unit: V elements of the first half of the rotated dimensions of a head with the V of the second
+// half that turn with them (or V / 2 neighbouring pairs), so q_out may be q; or V elements that are only copied.  Bound by HBM where
+// tokens are many: every element is read once and written once, 16 bytes at a time where the layout allows it.  What a token's place
+// is takes a chain of dependent loads, so the first two units of every thread are on their way before it is known.
+template <class T, int V>
 __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p) {
+  constexpr int AHEAD = 2;
   const int t = blockIdx.x;
   __shared__ int s_pos;
   __shared__ long long s_row;
-  if (threadIdx.x == 0) {
-    int pos = -1;
-    long long row = -1;
-    const int b = p.cu ? packed_find(p.cu, p.kv.batch, t) : t;
-    if (b >= 0) {
-      const int len = p.kv.lens[b];
-      if (p.cu) {
-        int begin, end;
-        bool bad = false;
-        packed_range(p.cu, b, p.tokens, &begin, &end, &bad);
-        pos = bad ? -1 : len - (end - t);
-      } else {
-        pos = len - 1;
-      }
-      if (pos >= 0 && (p.half == 0 || pos < p.max_position)) row = paged_row(p.kv, b, pos);
-      if (row < 0 && !(p.cu == nullptr && len == 0)) report(p.status, DEV_BAD_INDEX);
+  const T *q = static_cast<const T *>(p.q) + t * p.ldq;
+  const T *k = static_cast<const T *>(p.k) + t * p.ldk;
+  const T *v = static_cast<const T *>(p.v) + t * p.ldv;
+  const bool single = V == 1 && p.interleaved;                    // neighbours in pieces of their own
+  const int gap = single ? 1 : p.half;                            // from a piece to the one that turns with it
+  const int pairs = p.interleaved && !single ? 0 : p.half / V;    // units of a head that hold two pieces
+  const int units = p.dim / V - pairs, plain = p.dim / V;         // units of a head of q or k; of v
+  const int turned = (p.heads + p.kv_heads) * units, all = turned + p.kv_heads * plain;
+  struct Unit {
+    int head, at;        // head: queries, then keys, then values; first element inside the head
+    bool two;
+  };
+  auto unit = [&](int i) {
+    Unit u;
+    if (i < turned) {
+      u.head = i / units;
+      const int w = i - u.head * units;
+      u.two = w < pairs;
+      u.at = u.two ? w * (single ? 2 : V) : (w + pairs) * V;
+    } else {
+      i -= turned;
+      u.head = i / plain;
+      u.at = (i - u.head * plain) * V;
+      u.head += p.heads + p.kv_heads;
+      u.two = false;
     }
-    s_pos = pos;
-    s_row = row;
+    return u;
+  };
+  auto source = [&](const Unit &u) {
+    const int h = u.head;
+    return h < p.heads ? q + h * p.dim : h < p.heads + p.kv_heads ? k + (h - p.heads) * p.dim : v + (h - p.heads - p.kv_heads) * p.dim;
+  };
+  Piece<T, V> a[AHEAD], b[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) {
+    const int i = threadIdx.x + j * 256;
+    if (i < all) {
+      const Unit u = unit(i);
+      const T *src = source(u) + u.at;
+      a[j] = *reinterpret_cast<const Piece<T, V> *>(src);
+      if (u.two) b[j] = *reinterpret_cast<const Piece<T, V> *>(src + gap);
+    }
+  }
+  if (threadIdx.x < 32) {
+    int pos = -1;
+    const long long row = find_place(p, t, &pos);
+    if (threadIdx.x == 0) {
+      s_pos = pos;
+      s_row = row;
+    }
   }
   __syncthreads();
   const int pos = s_pos;
   const long long row = s_row;
   if (row < 0) return;
-  const T *q = static_cast<const T *>(p.q) + t * p.ldq;
-  const T *k = static_cast<const T *>(p.k) + t * p.ldk;
-  const T *v = static_cast<const T *>(p.v) + t * p.ldv;
   T *qo = static_cast<T *>(p.q_out) + t * p.ldqo;
   T *ko = p.k_out ? static_cast<T *>(p.k_out) + t * p.ldko : nullptr;
   T *ck = static_cast<T *>(p.cache_k) + row, *cv = static_cast<T *>(p.cache_v) + row;
   const float *cs = p.cos + (long long)pos * p.half, *sn = p.sin + (long long)pos * p.half;
-  const int units = p.dim - p.half;   // per head: the pairs, then the dimensions that stay
-  const int turned = (p.heads + p.kv_heads) * units;
-  for (int i = threadIdx.x; i < turned; i += blockDim.x) {
-    const int h = i / units, u = i % units;
-    const bool key = h >= p.heads;
-    const int kh = h - p.heads;
-    const T *src = key ? k + kh * p.dim : q + h * p.dim;
-    T *dst = key ? ck + kh * p.kv.head_stride : qo + h * p.dim;
-    T *dst2 = key && ko ? ko + kh * p.dim : nullptr;
-    if (u < p.half) {
-      const int a = p.interleaved ? 2 * u : u, b = p.interleaved ? 2 * u + 1 : u + p.half;
-      const float x = to_f32(src[a]), y = to_f32(src[b]);
-      const float c = cs[u], s = sn[u];
-      const float x1 = x * c - y * s, y1 = y * c + x * s;
-      from_f32(dst + a, x1);
-      from_f32(dst + b, y1);
-      if (dst2) { from_f32(dst2 + a, x1); from_f32(dst2 + b, y1); }
-    } else {
-      const int a = u + p.half;
-      const T x = src[a];
-      dst[a] = x;
-      if (dst2) dst2[a] = x;
+  auto finish = [&](const Unit &u, Piece<T, V> x, Piece<T, V> y) {
+    const int kh = u.head - p.heads, vh = kh - p.kv_heads;
+    T *dst = kh < 0 ? qo + u.head * p.dim : vh < 0 ? ck + kh * p.kv.head_stride : cv + vh * p.kv.head_stride;
+    T *dst2 = kh >= 0 && vh < 0 && ko ? ko + kh * p.dim : nullptr;
+    if (u.two) {
+      const int angle = single ? u.at / 2 : u.at;
+      const Piece<float, V> c = *reinterpret_cast<const Piece<float, V> *>(cs + angle), s = *reinterpret_cast<const Piece<float, V> *>(sn + angle);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float f = to_f32(x.x[e]), g = to_f32(y.x[e]);
+        from_f32(&x.x[e], f * c.x[e] - g * s.x[e]);
+        from_f32(&y.x[e], g * c.x[e] + f * s.x[e]);
+      }
+      *reinterpret_cast<Piece<T, V> *>(dst + u.at + gap) = y;
+      if (dst2) *reinterpret_cast<Piece<T, V> *>(dst2 + u.at + gap) = y;
+    } else if constexpr (V >= 2) {   // pairs of neighbours inside the piece
+      if (p.interleaved && vh < 0 && u.at < 2 * p.half) {
+        constexpr int W = V / 2;
+        const Piece<float, W> c = *reinterpret_cast<const Piece<float, W> *>(cs + u.at / 2), s = *reinterpret_cast<const Piece<float, W> *>(sn + u.at / 2);
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const float f = to_f32(x.x[2 * e]), g = to_f32(x.x[2 * e + 1]);
+          from_f32(&x.x[2 * e], f * c.x[e] - g * s.x[e]);
+          from_f32(&x.x[2 * e + 1], g * c.x[e] + f * s.x[e]);
+        }
+      }
     }
+    *reinterpret_cast<Piece<T, V> *>(dst + u.at) = x;
+    if (dst2) *reinterpret_cast<Piece<T, V> *>(dst2 + u.at) = x;
+  };
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) {
+    const int i = threadIdx.x + j * 256;
+    if (i < all) finish(unit(i), a[j], b[j]);
   }
-  for (int i = threadIdx.x; i < p.kv_heads * p.dim; i += blockDim.x) {
-    const int h = i / p.dim, d = i % p.dim;
-    cv[h * p.kv.head_stride + d] = v[i];
+  for (int i = threadIdx.x + AHEAD * 256; i < all; i += 256) {
+    const Unit u = unit(i);
+    const T *src = source(u) + u.at;
+    Piece<T, V> x = *reinterpret_cast<const Piece<T, V> *>(src), y;
+    if (u.two) y = *reinterpret_cast<const Piece<T, V> *>(src + gap);
+    finish(u, x, y);
+  }
+}
+
+// The widest piece that divides every extent and stride and to which every tensor is aligned.  10,832 tokens of 32 + 2 x 8 heads of 128
+// in bf16: 16-byte pieces MEASURED_VEC, single elements 131 us.
+static int widest_piece(const AppendParams &p, int es) {
+  uint64_t bits = (uint64_t)p.dim | (uint64_t)p.ldq | (uint64_t)p.ldk | (uint64_t)p.ldv | (uint64_t)p.ldqo | (uint64_t)p.ldko | (uint64_t)p.kv.page_stride |
+                  (uint64_t)p.kv.token_stride | (uint64_t)p.kv.head_stride | (uint64_t)(p.interleaved ? 2 * p.half : p.half);
+  uint64_t address = (uint64_t)(uintptr_t)p.q | (uint64_t)(uintptr_t)p.k | (uint64_t)(uintptr_t)p.v | (uint64_t)(uintptr_t)p.q_out | (uint64_t)(uintptr_t)p.k_out |
+                     (uint64_t)(uintptr_t)p.cache_k | (uint64_t)(uintptr_t)p.cache_v;
+  // angles come V (halves) or V / 2 (pairs) at a time, as fp32 and at most 16 bytes a load
+  const uint64_t angles = (uint64_t)(uintptr_t)p.cos | (uint64_t)(uintptr_t)p.sin;
+  for (int v = 16 / es; v > 1; v /= 2)
+    if (bits % v == 0 && address % (v * es) == 0 && angles % (p.interleaved ? v * 2 : v * 4) == 0) return v;
+  return 1;
+}
+
+template <class T>
+static void launch_append(cudaStream_t stream, const AppendParams &p, int v) {
+  const unsigned grid = (unsigned)p.tokens;
+  if (v == 8) {
+    if constexpr (sizeof(T) == 2) kv_append_kernel<T, 8><<<grid, 256, 0, stream>>>(p);
+  } else if (v == 4) {
+    kv_append_kernel<T, 4><<<grid, 256, 0, stream>>>(p);
+  } else if (v == 2) {
+    kv_append_kernel<T, 2><<<grid, 256, 0, stream>>>(p);
+  } else {
+    kv_append_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
   }
 }
 
@@ -188,8 +298,9 @@ extern "C" int sofie_b200_kv_append_enqueue(sofie_b200_ctx *ctx, const sofie_b20
   p.half = d.rotary_dim / 2; p.interleaved = d.interleaved != 0;
   p.max_position = d.max_position;
   p.status = ctx->d_status;
-  if (d.dtype == SOFIE_B200_F32) kv_append_kernel<float><<<(unsigned)d.tokens, 256, 0, ctx->stream>>>(p);
-  else kv_append_kernel<__nv_bfloat16><<<(unsigned)d.tokens, 256, 0, ctx->stream>>>(p);
+  const int piece = widest_piece(p, dtype_size(d.dtype));
+  if (d.dtype == SOFIE_B200_F32) launch_append<float>(ctx->stream, p, piece);
+  else launch_append<__nv_bfloat16>(ctx->stream, p, piece);
   SB_CUDA(cudaGetLastError());
   ctx->launches++;
   return 0;

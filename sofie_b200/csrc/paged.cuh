@@ -54,15 +54,14 @@ SB_HD void packed_range(const int32_t *cu, int b, long long rows, int *begin, in
   *end = y;
 }
 
-// The sequence that row t belongs to (cu[b] <= t < cu[b + 1]), or -1.  Any contents of cu end the search inside [0, batch).
-SB_HD int packed_find(const int32_t *cu, int batch, int t) {
-  int lo = 0, hi = batch;   // invariant for an ordered cu: cu[lo] <= t or no sequence holds t
-  while (hi - lo > 1) {
-    const int mid = lo + (hi - lo) / 2;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
-  }
-  return batch > 0 && cu[lo] <= t && t < cu[lo + 1] ? lo : -1;
+// The sequence that row t belongs to, cu[b] <= t < cu[b + 1], by a warp: of the sequences [lo, hi) that may hold it lane l looks at
+// search_probe (if that is below hi), and with k the highest lane that found cu <= t (0 if none did) search_narrow leaves a 32nd part.
+// From [0, batch) it ends at one sequence, to be checked, for any contents of cu.
+SB_HD int search_probe(int lo, int hi, int lane) { return lo + lane * ((hi - lo + 31) / 32); }
+SB_HD void search_narrow(int &lo, int &hi, int k) {
+  const int step = (hi - lo + 31) / 32;
+  lo += k * step;
+  if (hi > lo + step) hi = lo + step;
 }
 
 // ---- attention over the cache: dealing the work of a batch to blocks --------------------------------------------------

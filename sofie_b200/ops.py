@@ -190,8 +190,9 @@ class Context:
         [batch + 1], the packed rows of each sequence; absent = one token per sequence.  Token rows may be column blocks of a
         wider tensor.  q_out may be q, k_out may be k."""
         tokens, kv_heads, dim, ldk = _rows("k", k)
-        if (kv_heads, dim) != (kv.kv_heads, kv.head_dim) or k.dtype != kv.dtype:
-            raise ValueError(f"kv_append: keys of {kv_heads} heads of {dim} {k.dtype}, cache of {kv.kv_heads} of {kv.head_dim} {kv.dtype}")
+        dtype = k.dtype
+        if kv_heads != kv.kv_heads or dim != kv.head_dim or dtype is not kv.dtype:
+            raise ValueError(f"kv_append: keys of {kv_heads} heads of {dim} {dtype}, cache of {kv.kv_heads} of {kv.head_dim} {kv.dtype}")
         ldv = _same_rows("v", v, k)
         ldko = _same_rows("k_out", k_out, k) if k_out is not None else 0
         heads = ldq = ldqo = 0
@@ -199,24 +200,27 @@ class Context:
             if q_out is None:
                 raise ValueError("kv_append: q needs q_out")
             n, heads, qdim, ldq = _rows("q", q)
-            if n != tokens or qdim != dim or q.dtype != k.dtype:
+            if n != tokens or qdim != dim or q.dtype is not dtype:
                 raise ValueError("kv_append: q and k differ in tokens, head size or type")
             ldqo = _same_rows("q_out", q_out, q)
         elif q_out is not None:
             raise ValueError("kv_append: q_out needs q")
         rotary = positions = 0
         if cos is not None or sin is not None:
-            if cos is None or sin is None or cos.shape != sin.shape or cos.dim() != 2 or not (cos.is_contiguous() and sin.is_contiguous()):
+            if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
                 raise ValueError("kv_append: cos and sin are two contiguous tensors of one shape [positions, rotary_dim / 2]")
-            if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+            if cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
                 raise TypeError("kv_append: cos and sin are fp32")
-            positions, rotary = cos.shape[0], 2 * cos.shape[1]
+            positions, rotary = cos.shape
+            rotary *= 2
         if cu_seqlens is not None:
             _offsets("cu_seqlens", cu_seqlens, kv.batch)
-        d = L.KvAppendDesc(tokens, heads, kv_heads, dim, rotary, int(interleaved), dtype_code(k.dtype), positions, ldq, ldk, ldv, ldqo, ldko)
-        L.check(self._lib.sofie_b200_kv_append_enqueue(
+        d = L.KvAppendDesc(tokens, heads, kv_heads, dim, rotary, 1 if interleaved else 0, kv._dtype_code, positions, ldq, ldk, ldv, ldqo, ldko)
+        status = self._lib.sofie_b200_kv_append_enqueue(
             self._h, C.byref(d), kv._ref, _ptr(cu_seqlens), _ptr(q), _ptr(k), _ptr(v), _ptr(cos) if rotary else None, _ptr(sin) if rotary else None,
-            _ptr(q_out), _ptr(k_out)), "kv_append_enqueue")
+            _ptr(q_out), _ptr(k_out))
+        if status:
+            L.check(status, "kv_append_enqueue")
 
     def depth_unfold(self, x, y, taps, d_out, stride_d=1, pad_front=0, dil_d=1):
         """x [n, c, d, h, w] -> y [n * d_out, c * taps, h, w]: the depth taps of a 3-D convolution as channels."""
@@ -241,24 +245,25 @@ class Context:
 
 def _rows(name, t):
     """(tokens, heads, head size, token pitch) of a [tokens, heads, head_dim] tensor whose rows may be column blocks of wider ones."""
-    if t.dim() != 3:
-        raise ValueError(f"{name}: [tokens, heads, head_dim] is expected, not {tuple(t.shape)}")
-    n, h, d = t.shape
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{name}: [tokens, heads, head_dim] is expected, not {tuple(shape)}")
+    n, h, d = shape
     sn, sh, sd = t.stride()
-    if (d > 1 and sd != 1) or (h > 1 and sh != d):
+    if (sd != 1 and d > 1) or (sh != d and h > 1):
         raise ValueError(f"{name}: the heads of a token must lie one behind another (strides {t.stride()})")
     return n, h, d, sn if n > 1 else h * d
 
 
 def _same_rows(name, t, like):
     """Token pitch of `t`, which has the shape and type of `like`."""
-    if t.shape != like.shape or t.dtype != like.dtype:
+    if t.shape != like.shape or t.dtype is not like.dtype:
         raise ValueError(f"{name}: {tuple(like.shape)} {like.dtype} is expected, not {tuple(t.shape)} {t.dtype}")
     return _rows(name, t)[3]
 
 
 def _offsets(name, t, batch):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != batch + 1 or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != batch + 1 or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous int32 tensor of batch + 1 = {batch + 1} row offsets is expected")
 
 
@@ -283,6 +288,7 @@ class PagedKV:
             raise ValueError("PagedKV: all tensors live on one device")
         self.k, self.v, self.block_table, self.seq_lens = k, v, block_table, seq_lens
         self.kv_heads, self.head_dim, self.dtype, self.batch = kv_heads, dim, k.dtype, seq_lens.shape[0]
+        self._dtype_code = dtype_code(k.dtype)
         width = block_table.shape[1]
         # the stride of an axis of one element says nothing: the dense one stands for it
         hs = k.stride(2) if kv_heads > 1 else dim
@@ -321,7 +327,7 @@ class PromptAttentionPlan:
         cu_seqlens (and cu_seqlens_k, where keys have other lengths than queries): int32 [batch + 1] row offsets."""
         n, h, d, ldq = _rows("q", q)
         nk, hk, dk, ldk = _rows("k", k)
-        if (h, hk, d) != self._shape or dk != d or q.dtype != self._dtype or k.dtype != self._dtype:
+        if (h, hk, d) != self._shape or dk != d or q.dtype is not self._dtype or k.dtype is not self._dtype:
             raise ValueError(f"prompt attention: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype} do not match the plan")
         batch = cu_seqlens.shape[0] - 1
         if batch < 0:
@@ -329,9 +335,11 @@ class PromptAttentionPlan:
         _offsets("cu_seqlens", cu_seqlens, batch)
         if cu_seqlens_k is not None:
             _offsets("cu_seqlens_k", cu_seqlens_k, batch)
-        pitches = (ldq, ldk, _same_rows("v", v, k), _same_rows("y", y, q))
-        L.check(self._lib.sofie_b200_prompt_attention_enqueue(self._plan(pitches), _ptr(q), _ptr(k), _ptr(v), _ptr(y), _ptr(cu_seqlens),
-                                                              _ptr(cu_seqlens_k), batch, n, nk), "prompt_attention_enqueue")
+        status = self._lib.sofie_b200_prompt_attention_enqueue(
+            self._plan((ldq, ldk, _same_rows("v", v, k), _same_rows("y", y, q))), _ptr(q), _ptr(k), _ptr(v), _ptr(y), _ptr(cu_seqlens),
+            _ptr(cu_seqlens_k), batch, n, nk)
+        if status:
+            L.check(status, "prompt_attention_enqueue")
 
     def close(self) -> None:
         for h in self._plans.values():
@@ -379,11 +387,12 @@ class PagedAttentionPlan:
     def enqueue(self, q, kv, y) -> None:
         """q, y: [batch, heads, head_dim]; kv: the PagedKV with the cache and its batch of sequences."""
         n, h, d, ldq = _rows("q", q)
-        if (h, kv.kv_heads, d) != self._shape or kv.head_dim != d or q.dtype != self._dtype or kv.dtype != self._dtype or n != kv.batch:
+        if (h, kv.kv_heads, d) != self._shape or kv.head_dim != d or q.dtype is not self._dtype or kv.dtype is not self._dtype or n != kv.batch:
             raise ValueError(f"paged attention: q {tuple(q.shape)} {q.dtype} over {kv.batch} sequences of {kv.kv_heads} heads of {kv.head_dim} "
                              f"{kv.dtype} does not match the plan")
-        L.check(self._lib.sofie_b200_paged_attention_enqueue(self._plan((ldq, _same_rows("y", y, q))), _ptr(q), kv._ref, _ptr(y),
-                                                             _ptr(self._workspace)), "paged_attention_enqueue")
+        status = self._lib.sofie_b200_paged_attention_enqueue(self._plan((ldq, _same_rows("y", y, q))), _ptr(q), kv._ref, _ptr(y), _ptr(self._workspace))
+        if status:
+            L.check(status, "paged_attention_enqueue")
 
     def close(self) -> None:
         for h in self._plans.values():

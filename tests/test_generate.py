@@ -182,7 +182,7 @@ int main() {
   }
   // packed rows: a range is inside the tensor or refused; a row's sequence holds the row
   for (int it = 0; it < 50000; ++it) {
-    const int batch = 1 + rnd(8), rows = rnd(40);
+    const int batch = 1 + rnd(it % 50 ? 8 : 3000), rows = rnd(40);
     std::vector<int> cu(batch + 1);
     const bool ordered = rnd(2);
     int at = 0;
@@ -195,10 +195,18 @@ int main() {
       NEED(bad || (x == cu[b] && y == cu[b + 1]));
     }
     for (int t = 0; t < rows; ++t) {
-      const int b = packed_find(cu.data(), batch, t);
-      NEED(b >= -1 && b < batch);
-      if (b >= 0) NEED(cu[b] <= t && t < cu[b + 1]);
-      if (ordered) NEED((b >= 0) == (t >= cu[0] && t < cu[batch]));
+      int lo = 0, hi = batch, rounds = 0;
+      while (hi - lo > 1) {
+        int k = 0;
+        for (int lane = 0; lane < 32; ++lane) {
+          const int at = search_probe(lo, hi, lane);
+          if (at < hi && cu[at] <= t) k = lane;
+        }
+        search_narrow(lo, hi, k);
+        NEED(lo >= 0 && lo < hi && hi <= batch && ++rounds < 8);
+      }
+      const bool found = cu[lo] <= t && t < cu[lo + 1];
+      if (ordered) NEED(found == (t >= cu[0] && t < cu[batch]));
     }
   }
   puts("ok");
