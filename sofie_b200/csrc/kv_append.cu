@@ -73,34 +73,39 @@ struct AppendParams {
   int *status;
 };
 
-// Position of token t and the element offset of its place in the cache (negative: no place, the token is left out), found by a warp:
-// 32 offsets of cu_seqlens at a time, so two rounds of loads for a thousand sequences.
-__device__ __forceinline__ long long find_place(const AppendParams &p, int t, int *pos_out) {
+// Position of token t in its sequence (and which that is), found by a warp: 32 sequences at a time, their offsets and lengths side by
+// side, so that one round of loads does for up to 32 sequences and two for a thousand.  Negative: the token has no place, and `bad` says
+// whether that is an error (a row behind the last sequence and a padding row are none).
+__device__ __forceinline__ int find_position(const AppendParams &p, int t, int *seq, bool *bad) {
   const int lane = threadIdx.x & 31;
-  int b = t;
-  if (p.cu) {
-    int lo = 0, hi = p.kv.batch;
-    while (hi - lo > 1) {
-      const int at = search_probe(lo, hi, lane);
-      const uint32_t below = __ballot_sync(0xffffffffu, at < hi && p.cu[at] <= t);
-      search_narrow(lo, hi, below ? 31 - __clz(below) : 0);
-    }
-    b = p.cu[lo] <= t && t < p.cu[lo + 1] ? lo : -1;
+  *bad = false;
+  *seq = t;
+  if (!p.cu) {
+    const int len = p.kv.lens[t];
+    *bad = len < 0;
+    return len - 1;
   }
-  if (b < 0) return -1;
-  const int len = p.kv.lens[b];
-  int pos = len - 1;
-  if (p.cu) {
-    int begin, end;
-    bool bad = false;
-    packed_range(p.cu, b, p.tokens, &begin, &end, &bad);
-    pos = bad ? -1 : len - (end - t);
+  int lo = 0, hi = p.kv.batch;
+  while (hi - lo > 32) {
+    const int at = search_probe(lo, hi, lane);
+    const uint32_t below = __ballot_sync(0xffffffffu, at < hi && p.cu[at] <= t);
+    search_narrow(lo, hi, below ? 31 - __clz(below) : 0);
   }
-  long long row = -1;
-  if (pos >= 0 && (p.half == 0 || pos < p.max_position)) row = paged_row(p.kv, b, pos);
-  if (row < 0 && !(p.cu == nullptr && len == 0) && lane == 0) report(p.status, DEV_BAD_INDEX);
-  *pos_out = pos;
-  return row;
+  int begin = 0, end = 0, len = 0;
+  if (lo + lane < hi) {
+    begin = p.cu[lo + lane];
+    end = p.cu[lo + lane + 1];
+    len = p.kv.lens[lo + lane];
+  }
+  const uint32_t here = __ballot_sync(0xffffffffu, begin <= t && t < end);
+  if (!here) return -1;
+  const int src = __ffs(here) - 1;
+  begin = __shfl_sync(0xffffffffu, begin, src);
+  end = __shfl_sync(0xffffffffu, end, src);
+  len = __shfl_sync(0xffffffffu, len, src);
+  *seq = lo + src;
+  *bad = begin < 0 || end > p.tokens || len < end - t;
+  return *bad ? -1 : len - (end - t);
 }
 
 // A piece of V elements as they lie in memory (V * sizeof(T) = 16, 8, 4 or 2 bytes).
@@ -109,121 +114,158 @@ struct alignas(sizeof(T) * V) Piece {
   T x[V];
 };
 
-// One block per token, a thread per unit: V elements of the first half of the rotated dimensions of a head with the V of the second
-// half that turn with them (or V / 2 neighbouring pairs), so q_out may be q; or V elements that are only copied.  Bound by HBM where
-// tokens are many: every element is read once and written once, 16 bytes at a time where the layout allows it.  What a token's place
-// is takes a chain of dependent loads, so the first two units of every thread are on their way before it is known.
-template <class T, int V>
-__global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p) {
-  constexpr int AHEAD = 2;
-  const int t = blockIdx.x;
-  __shared__ int s_pos;
-  __shared__ long long s_row;
-  const T *q = static_cast<const T *>(p.q) + t * p.ldq;
-  const T *k = static_cast<const T *>(p.k) + t * p.ldk;
-  const T *v = static_cast<const T *>(p.v) + t * p.ldv;
+// GROUP threads per token (a block or two warps).  A unit of a query or key head is V elements of the first half of its rotated dimensions
+// with the V of the second half that turn with them (or V / 2 neighbouring pairs), so q_out may be q; or V elements that are only
+// copied.  A thread has the same unit of several heads, so its angles are loaded once.  Bound by HBM where tokens are many: every element
+// is read once and written once, 16 bytes at a time where the layout allows it; what keeps it from the copy rate is that a thread
+// waits for its loads, two heads at a time (more take registers, and with them warps: 4 heads 79 us, 2 heads 63 us at 10,832 tokens of
+// 32 + 2 x 8 heads of 128 in bf16 = 4.3 TB/s).  The first heads are on their way before the token's place is known, which takes two or
+// three rounds of dependent loads.
+template <class T, int V, int GROUP>
+__global__ void __launch_bounds__(256, GROUP < 256 ? 4 : 1) kv_append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int AHEAD = 2;   // heads under way, and pieces of values
+  typedef Piece<T, V> P;
+  const int t = blockIdx.x * (256 / GROUP) + threadIdx.x / GROUP, me = threadIdx.x % GROUP;
+  if (GROUP < 256 && t >= p.tokens) return;
   const bool single = V == 1 && p.interleaved;                    // neighbours in pieces of their own
   const int gap = single ? 1 : p.half;                            // from a piece to the one that turns with it
   const int pairs = p.interleaved && !single ? 0 : p.half / V;    // units of a head that hold two pieces
-  const int units = p.dim / V - pairs, plain = p.dim / V;         // units of a head of q or k; of v
-  const int turned = (p.heads + p.kv_heads) * units, all = turned + p.kv_heads * plain;
-  struct Unit {
-    int head, at;        // head: queries, then keys, then values; first element inside the head
-    bool two;
+  const int units = p.dim / V - pairs, heads = p.heads + p.kv_heads;
+  const int side = units < GROUP ? GROUP / units : 1;             // heads side by side
+  const int first = units < GROUP ? me / units : 0;               // this thread's first head
+  int u = units < GROUP ? me - first * units : me;                // its unit; with more units than threads also u + GROUP, ...
+  const bool works = first < side && u < units;
+  const T *q = static_cast<const T *>(p.q) + t * p.ldq;
+  const T *k = static_cast<const T *>(p.k) + t * p.ldk - p.heads * p.dim;   // heads counted on from the queries'
+  const T *v = static_cast<const T *>(p.v) + t * p.ldv;
+  const int pieces = p.dim / V, values = p.kv_heads * pieces;
+  P x[AHEAD], y[AHEAD], w[AHEAD];
+  Piece<float, V> c, sn;
+  bool two, inside;
+  int at;
+  auto choose = [&]() {
+    two = u < pairs;
+    at = two ? u * (single ? 2 : V) : (u + pairs) * V;
+    inside = V > 1 && p.interleaved && at < 2 * p.half;   // pairs of neighbours inside the piece
   };
-  auto unit = [&](int i) {
-    Unit u;
-    if (i < turned) {
-      u.head = i / units;
-      const int w = i - u.head * units;
-      u.two = w < pairs;
-      u.at = u.two ? w * (single ? 2 : V) : (w + pairs) * V;
-    } else {
-      i -= turned;
-      u.head = i / plain;
-      u.at = (i - u.head * plain) * V;
-      u.head += p.heads + p.kv_heads;
-      u.two = false;
-    }
-    return u;
-  };
-  auto source = [&](const Unit &u) {
-    const int h = u.head;
-    return h < p.heads ? q + h * p.dim : h < p.heads + p.kv_heads ? k + (h - p.heads) * p.dim : v + (h - p.heads - p.kv_heads) * p.dim;
-  };
-  Piece<T, V> a[AHEAD], b[AHEAD];
+  auto angles = [&](int pos) {
+    const float *cs = p.cos + (long long)pos * p.half, *ss = p.sin + (long long)pos * p.half;
+    if (two) {
+      c = *reinterpret_cast<const Piece<float, V> *>(cs + (single ? at / 2 : at));
+      sn = *reinterpret_cast<const Piece<float, V> *>(ss + (single ? at / 2 : at));
+    } else if (inside) {
+      constexpr int W = V > 1 ? V / 2 : 1;
+      const Piece<float, W> cw = *reinterpret_cast<const Piece<float, W> *>(cs + at / 2), sw = *reinterpret_cast<const Piece<float, W> *>(ss + at / 2);
 #pragma unroll
-  for (int j = 0; j < AHEAD; ++j) {
-    const int i = threadIdx.x + j * 256;
-    if (i < all) {
-      const Unit u = unit(i);
-      const T *src = source(u) + u.at;
-      a[j] = *reinterpret_cast<const Piece<T, V> *>(src);
-      if (u.two) b[j] = *reinterpret_cast<const Piece<T, V> *>(src + gap);
+      for (int e = 0; e < W; ++e) c.x[e] = cw.x[e], sn.x[e] = sw.x[e];
     }
-  }
-  if (threadIdx.x < 32) {
-    int pos = -1;
-    const long long row = find_place(p, t, &pos);
-    if (threadIdx.x == 0) {
-      s_pos = pos;
-      s_row = row;
-    }
-  }
-  __syncthreads();
-  const int pos = s_pos;
-  const long long row = s_row;
-  if (row < 0) return;
-  T *qo = static_cast<T *>(p.q_out) + t * p.ldqo;
-  T *ko = p.k_out ? static_cast<T *>(p.k_out) + t * p.ldko : nullptr;
-  T *ck = static_cast<T *>(p.cache_k) + row, *cv = static_cast<T *>(p.cache_v) + row;
-  const float *cs = p.cos + (long long)pos * p.half, *sn = p.sin + (long long)pos * p.half;
-  auto finish = [&](const Unit &u, Piece<T, V> x, Piece<T, V> y) {
-    const int kh = u.head - p.heads, vh = kh - p.kv_heads;
-    T *dst = kh < 0 ? qo + u.head * p.dim : vh < 0 ? ck + kh * p.kv.head_stride : cv + vh * p.kv.head_stride;
-    T *dst2 = kh >= 0 && vh < 0 && ko ? ko + kh * p.dim : nullptr;
-    if (u.two) {
-      const int angle = single ? u.at / 2 : u.at;
-      const Piece<float, V> c = *reinterpret_cast<const Piece<float, V> *>(cs + angle), s = *reinterpret_cast<const Piece<float, V> *>(sn + angle);
+  };
+  auto take = [&](int h) {   // heads h, h + side, ...
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float f = to_f32(x.x[e]), g = to_f32(y.x[e]);
-        from_f32(&x.x[e], f * c.x[e] - g * s.x[e]);
-        from_f32(&y.x[e], g * c.x[e] + f * s.x[e]);
+    for (int j = 0; j < AHEAD; ++j) {
+      const int hh = h + j * side;
+      if (hh < heads) {
+        const T *src = (hh < p.heads ? q : k) + hh * p.dim + at;
+        x[j] = *reinterpret_cast<const P *>(src);
+        if (two) y[j] = *reinterpret_cast<const P *>(src + gap);
       }
-      *reinterpret_cast<Piece<T, V> *>(dst + u.at + gap) = y;
-      if (dst2) *reinterpret_cast<Piece<T, V> *>(dst2 + u.at + gap) = y;
-    } else if constexpr (V >= 2) {   // pairs of neighbours inside the piece
-      if (p.interleaved && vh < 0 && u.at < 2 * p.half) {
-        constexpr int W = V / 2;
-        const Piece<float, W> c = *reinterpret_cast<const Piece<float, W> *>(cs + u.at / 2), s = *reinterpret_cast<const Piece<float, W> *>(sn + u.at / 2);
+    }
+  };
+  auto take_values = [&](int i0) {
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const float f = to_f32(x.x[2 * e]), g = to_f32(x.x[2 * e + 1]);
-          from_f32(&x.x[2 * e], f * c.x[e] - g * s.x[e]);
-          from_f32(&x.x[2 * e + 1], g * c.x[e] + f * s.x[e]);
+    for (int j = 0; j < AHEAD; ++j)
+      if (i0 + j * GROUP < values) w[j] = *reinterpret_cast<const P *>(v + (i0 + j * GROUP) * V);
+  };
+  choose();
+  if (works) take(first);
+  take_values(me);
+
+  int pos, seq;
+  bool bad;
+  if (GROUP < 256) {   // every warp for itself
+    pos = find_position(p, t, &seq, &bad);
+  } else {
+    __shared__ int s_pos, s_seq;
+    __shared__ bool s_bad;
+    if (threadIdx.x < 32) {
+      pos = find_position(p, t, &seq, &bad);
+      if (threadIdx.x == 0) s_pos = pos, s_seq = seq, s_bad = bad;
+    }
+    __syncthreads();
+    pos = s_pos, seq = s_seq, bad = s_bad;
+  }
+  long long row = -1;
+  if (pos >= 0) {
+    if (p.half && pos >= p.max_position) {
+      bad = true;
+    } else {
+      if (works) angles(pos);
+      row = paged_row(p.kv, seq, pos);
+      bad = row < 0;
+    }
+  }
+  if (row < 0) {
+    if (bad && me == 0) report(p.status, DEV_BAD_INDEX);
+    return;
+  }
+  if (works) {
+    T *qo = static_cast<T *>(p.q_out) + t * p.ldqo;
+    T *ko = p.k_out ? static_cast<T *>(p.k_out) + t * p.ldko - p.heads * p.dim : nullptr;
+    T *ck = static_cast<T *>(p.cache_k) + row - p.heads * p.kv.head_stride;
+    for (bool begun = true;; begun = false) {
+      for (int h = first; h < heads; h += AHEAD * side) {
+        if (!begun || h != first) take(h);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+          const int hh = h + j * side;
+          if (hh < heads) {
+            T *dst = hh < p.heads ? qo + hh * p.dim : ck + hh * p.kv.head_stride;
+            T *dst2 = hh >= p.heads && ko ? ko + hh * p.dim : nullptr;
+            if (two) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) {
+                const float f = to_f32(x[j].x[e]), g = to_f32(y[j].x[e]);
+                from_f32(&x[j].x[e], f * c.x[e] - g * sn.x[e]);
+                from_f32(&y[j].x[e], g * c.x[e] + f * sn.x[e]);
+              }
+              *reinterpret_cast<P *>(dst + at + gap) = y[j];
+              if (dst2) *reinterpret_cast<P *>(dst2 + at + gap) = y[j];
+            } else if (inside) {
+#pragma unroll
+              for (int e = 0; e + 1 < V; e += 2) {
+                const float f = to_f32(x[j].x[e]), g = to_f32(x[j].x[e + 1]);
+                from_f32(&x[j].x[e], f * c.x[e / 2] - g * sn.x[e / 2]);
+                from_f32(&x[j].x[e + 1], g * c.x[e / 2] + f * sn.x[e / 2]);
+              }
+            }
+            *reinterpret_cast<P *>(dst + at) = x[j];
+            if (dst2) *reinterpret_cast<P *>(dst2 + at) = x[j];
+          }
         }
       }
+      u += GROUP;
+      if (u >= units || units < GROUP) break;
+      choose();
+      angles(pos);
     }
-    *reinterpret_cast<Piece<T, V> *>(dst + u.at) = x;
-    if (dst2) *reinterpret_cast<Piece<T, V> *>(dst2 + u.at) = x;
-  };
-#pragma unroll
-  for (int j = 0; j < AHEAD; ++j) {
-    const int i = threadIdx.x + j * 256;
-    if (i < all) finish(unit(i), a[j], b[j]);
   }
-  for (int i = threadIdx.x + AHEAD * 256; i < all; i += 256) {
-    const Unit u = unit(i);
-    const T *src = source(u) + u.at;
-    Piece<T, V> x = *reinterpret_cast<const Piece<T, V> *>(src), y;
-    if (u.two) y = *reinterpret_cast<const Piece<T, V> *>(src + gap);
-    finish(u, x, y);
+  // the values, as they are
+  T *cv = static_cast<T *>(p.cache_v) + row;
+  for (int i0 = me; i0 < values; i0 += AHEAD * GROUP) {
+    if (i0 != me) take_values(i0);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int i = i0 + j * GROUP;
+      if (i < values) {
+        const int h = i / pieces;
+        *reinterpret_cast<P *>(cv + h * p.kv.head_stride + (i - h * pieces) * V) = w[j];
+      }
+    }
   }
 }
 
 // The widest piece that divides every extent and stride and to which every tensor is aligned.  10,832 tokens of 32 + 2 x 8 heads of 128
-// in bf16: 16-byte pieces MEASURED_VEC, single elements 131 us.
+// in bf16: 16-byte pieces 63 us, single elements 131 us.
 static int widest_piece(const AppendParams &p, int es) {
   uint64_t bits = (uint64_t)p.dim | (uint64_t)p.ldq | (uint64_t)p.ldk | (uint64_t)p.ldv | (uint64_t)p.ldqo | (uint64_t)p.ldko | (uint64_t)p.kv.page_stride |
                   (uint64_t)p.kv.token_stride | (uint64_t)p.kv.head_stride | (uint64_t)(p.interleaved ? 2 * p.half : p.half);
@@ -236,17 +278,23 @@ static int widest_piece(const AppendParams &p, int es) {
   return 1;
 }
 
+template <class T, int V>
+static void launch_append(sofie_b200_ctx *ctx, const AppendParams &p) {
+  // Few tokens: a block each, for the shortest way (120 tokens of 32 + 2 x 8 heads of 128: as long as an empty launch either way).  From
+  // four for every SM on: two warps each, four tokens to a block; of 10,832 tokens a block takes 101 us, four warps 70, two 63, one 68.
+  if (p.tokens < ctx->sm_count * 4) kv_append_kernel<T, V, 256><<<(unsigned)p.tokens, 256, 0, ctx->stream>>>(p);
+  else kv_append_kernel<T, V, 64><<<(unsigned)((p.tokens + 3) / 4), 256, 0, ctx->stream>>>(p);
+}
 template <class T>
-static void launch_append(cudaStream_t stream, const AppendParams &p, int v) {
-  const unsigned grid = (unsigned)p.tokens;
+static void launch_append(sofie_b200_ctx *ctx, const AppendParams &p, int v) {
   if (v == 8) {
-    if constexpr (sizeof(T) == 2) kv_append_kernel<T, 8><<<grid, 256, 0, stream>>>(p);
+    if constexpr (sizeof(T) == 2) launch_append<T, 8>(ctx, p);
   } else if (v == 4) {
-    kv_append_kernel<T, 4><<<grid, 256, 0, stream>>>(p);
+    launch_append<T, 4>(ctx, p);
   } else if (v == 2) {
-    kv_append_kernel<T, 2><<<grid, 256, 0, stream>>>(p);
+    launch_append<T, 2>(ctx, p);
   } else {
-    kv_append_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
+    launch_append<T, 1>(ctx, p);
   }
 }
 
@@ -299,8 +347,8 @@ extern "C" int sofie_b200_kv_append_enqueue(sofie_b200_ctx *ctx, const sofie_b20
   p.max_position = d.max_position;
   p.status = ctx->d_status;
   const int piece = widest_piece(p, dtype_size(d.dtype));
-  if (d.dtype == SOFIE_B200_F32) launch_append<float>(ctx->stream, p, piece);
-  else launch_append<__nv_bfloat16>(ctx->stream, p, piece);
+  if (d.dtype == SOFIE_B200_F32) launch_append<float>(ctx, p, piece);
+  else launch_append<__nv_bfloat16>(ctx, p, piece);
   SB_CUDA(cudaGetLastError());
   ctx->launches++;
   return 0;
