@@ -64,31 +64,69 @@ SB_HD void search_narrow(int &lo, int &hi, int k) {
   if (hi > lo + step) hi = lo + step;
 }
 
-// ---- attention over the cache: dealing the work of a batch to blocks --------------------------------------------------
-// The work is a row of equal units (`unit` keys of one key head of one sequence), ordered by sequence, then head, then key; block c of
-// `blocks` takes the units [split_at(U, blocks, c), split_at(U, blocks, c + 1)).  Shares differ by one unit at most, whatever
-// the lengths are.  A part of an item (one head of one sequence) that is not the whole of it goes to a slot of the workspace:
-// slot 0 of its block when the item began in an earlier block, slot 1 when it begins here and goes on.  A block has at most one of each.
-SB_HD long long split_at(long long units, int blocks, int c) { return units / blocks * c + units % blocks * c / blocks; }
+// ---- attention over the cache: dealing the work of a batch to workers (warps) ------------------------------------------
+// An item is one head of one sequence; it takes ITEM_COST slots (what beginning and ending one costs, in units of time) and then one
+// slot for every unit of `unit` keys.  The slots of all items, ordered by sequence, then head, then key, are one row; worker c of
+// `workers` takes the slots [split_at(S, workers, c), split_at(S, workers, c + 1)).  Shares differ by one slot at most, whatever the lengths
+// are.  A part of an item that is not the whole of it goes to a place of the workspace: place 0 of its worker when the item began
+// in an earlier one, place 1 when it begins here and goes on.  A worker has at most one of each.
+constexpr int ITEM_COST = 1;
 
-// The last block that holds a unit before `end`, 0 < end <= units.
-SB_HD int split_last(long long units, int blocks, long long end) {
-  int lo = 0, hi = blocks - 1;   // the largest c with split_at(c) < end
+SB_HD long long split_at(long long slots, int workers, int c) { return slots / workers * c + slots % workers * c / workers; }
+
+// The last worker that holds a slot before `end`, 0 < end <= slots.
+SB_HD int split_last(long long slots, int workers, long long end) {
+  int lo = 0, hi = workers - 1;   // the largest c with split_at(c) < end
   while (lo < hi) {
     const int mid = lo + (hi - lo + 1) / 2;
-    if (split_at(units, blocks, mid) < end) lo = mid;
+    if (split_at(slots, workers, mid) < end) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
 
-// Blocks that get work: no block fewer than `least` units, unless there are fewer in all.
-SB_HD int split_blocks(long long units, int blocks, int least) {
-  const long long most = (units + least - 1) / least;
-  return most < 1 ? 1 : most < blocks ? (int)most : blocks;
+// Workers that get work: none fewer than `least` slots, unless there are fewer in all.
+SB_HD int split_workers(long long slots, int workers, int least) {
+  const long long most = (slots + least - 1) / least;
+  return most < 1 ? 1 : most < workers ? (int)most : workers;
 }
 
 // Units of a sequence of n tokens.
 SB_HD int units_of(int n, int unit) { return (int)(((long long)n + unit - 1) / unit); }
+
+// Slots of all items of a sequence.
+SB_HD long long slots_of(int n, int unit, int items) { return n > 0 ? ((long long)units_of(n, unit) + ITEM_COST) * items : 0; }
+
+// A worker's way down its share.  left: slots of the share from `unit` on; nothing is left when it is 0 or less.
+struct Cursor {
+  int b, item, unit, units, len;   // sequence, item of the sequence, unit of the item; units and tokens of the sequence
+  long long left;
+};
+
+// From slot `offset` of the items of sequence c.b (whose len is set) on.
+SB_HD void cursor_start(Cursor &c, long long offset, int unit) {
+  c.units = units_of(c.len, unit);
+  const long long per = (long long)c.units + ITEM_COST;
+  c.item = (int)(offset / per);
+  const long long o = offset % per;
+  c.unit = o > ITEM_COST ? (int)(o - ITEM_COST) : 0;
+  if (o < ITEM_COST) c.left -= ITEM_COST - o;
+}
+
+// The next unit; lens[] is read where a sequence ends.
+SB_HD void cursor_next(Cursor &c, const PagedView &kv, int items, int unit) {
+  --c.left;
+  if (++c.unit < c.units) return;
+  c.unit = 0;
+  c.left -= ITEM_COST;
+  if (++c.item < items) return;
+  c.item = 0;
+  bool bad = false;
+  do {
+    ++c.b;
+  } while (c.b < kv.batch && (c.len = paged_len(kv, c.b, &bad)) == 0);
+  c.units = c.b < kv.batch ? units_of(c.len, unit) : 0;
+  if (c.b >= kv.batch) c.left = 0;
+}
 
 }  // namespace sb200

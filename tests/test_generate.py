@@ -239,61 +239,84 @@ using namespace sb200;
 static unsigned rs = 99;
 static int rnd(int n) { rs = rs * 1664525u + 1013904223u; return (int)((rs >> 8) % (unsigned)n); }
 int main() {
-  for (int it = 0; it < 4000; ++it) {
-    const int batch = 1 + rnd(12), items = 1 + rnd(9), unit = rnd(2) ? 64 : 32, grid = 1 + rnd(it % 2 ? 30 : 600), least = 1 + rnd(4);
-    std::vector<int> n(batch);
+  for (int it = 0; it < 3000; ++it) {
+    const int batch = 1 + rnd(12), items = 1 + rnd(9), unit = 16, all = 1 + rnd(it % 2 ? 30 : 600), least = 1 + rnd(8);
+    std::vector<int> n(batch), table(batch * 1000, 0);
     for (auto &x : n) x = rnd(4) ? rnd(it % 3 ? 700 : 9000) : rnd(2);
-    long long units = 0;
-    std::vector<long long> end;   // of each item in the row of units
+    PagedView kv{table.data(), n.data(), 1000, 16 * 8, 8, 8, batch, 1, 1000, 16};
+    long long slots = 0;
+    std::vector<long long> base(batch + 1);
+    for (int b = 0; b < batch; ++b) base[b] = slots, slots += slots_of(n[b], unit, items);
+    base[batch] = slots;
+    const int workers = split_workers(slots, all, least);
+    NEED(workers >= 1 && workers <= all && (workers == 1 || slots / workers >= 1));
+    std::vector<std::vector<int>> seen(batch * items);   // which worker took each unit
     for (int b = 0; b < batch; ++b)
-      for (int i = 0; i < items && n[b]; ++i) end.push_back(units += units_of(n[b], unit));
-    const int blocks = split_blocks(units, grid, least);
-    NEED(blocks >= 1 && blocks <= grid);
-    NEED(blocks == 1 || units / blocks >= 1);
-    std::vector<int> parts(end.size()), whole(end.size());
+      for (int i = 0; i < items; ++i) seen[b * items + i].assign(units_of(n[b], unit), -1);
     long long at = 0, lo = 1LL << 60, hi = 0;
-    for (int c = 0; c < blocks; ++c) {
-      const long long b = split_at(units, blocks, c), e = split_at(units, blocks, c + 1);
-      NEED(b == at && e >= b);
-      at = e;
-      lo = std::min(lo, e - b);
-      hi = std::max(hi, e - b);
-      int slot0 = 0, slot1 = 0;
-      for (size_t i = 0; i < end.size(); ++i) {
-        const long long first = i ? end[i - 1] : 0, s = std::max(b, first), t = std::min(e, end[i]);
-        if (s >= t) continue;
-        if (s == first && t == end[i]) { ++whole[i]; continue; }
-        ++parts[i];
-        if (s == first) {
-          ++slot1;
-          const int last = split_last(units, blocks, end[i]);
-          NEED(last > c && last < blocks);
-          NEED(split_at(units, blocks, last) < end[i] && split_at(units, blocks, last + 1) >= end[i]);
-        } else {
-          ++slot0;
+    struct Join { int b, item, parts; };
+    std::vector<Join> joins(workers, Join{0, 0, 0});
+    std::vector<int> place0(workers), place1(workers);
+    for (int c = 0; c < workers; ++c) {
+      const long long begin = split_at(slots, workers, c), end = split_at(slots, workers, c + 1);
+      NEED(begin == at && end >= begin);
+      at = end;
+      lo = std::min(lo, end - begin);
+      hi = std::max(hi, end - begin);
+      if (begin == end) continue;
+      int b = 0;
+      while (base[b + 1] <= begin) ++b;
+      Cursor k;
+      k.b = b;
+      k.len = n[b];
+      k.left = end - begin;
+      cursor_start(k, begin - base[b], unit);
+      while (k.left > 0) {   // a segment, as the kernels take it
+        NEED(k.b < batch && k.item < items && k.unit < k.units && k.len == n[k.b]);
+        const int first = k.unit, m = (int)std::min((long long)(k.units - k.unit), k.left);
+        for (int u = first; u < first + m; ++u) {
+          int &s = seen[k.b * items + k.item][u];
+          NEED(s == -1);
+          s = c;
         }
+        const bool begins = first == 0, ends = first + m == k.units;
+        if (!(begins && ends)) {
+          NEED((begins ? place1 : place0)[c]++ == 0);
+          if (begins) {
+            const long long item_end = end - k.left + k.units;
+            NEED(item_end == base[k.b] + (long long)(k.units + ITEM_COST) * (k.item + 1));
+            joins[c] = {k.b, k.item, split_last(slots, workers, item_end) - c + 1};
+            NEED(joins[c].parts >= 2 && c + joins[c].parts <= workers);
+          }
+        }
+        k.unit += m - 1;
+        k.left -= m - 1;
+        cursor_next(k, kv, items, unit);
       }
-      NEED(slot0 <= 1 && slot1 <= 1);
     }
-    NEED(at == units && (units == 0 || hi - lo <= 1));
-    for (size_t i = 0; i < end.size(); ++i) {
-      const long long first = i ? end[i - 1] : 0;
-      NEED((whole[i] == 1 && parts[i] == 0) || (whole[i] == 0 && parts[i] >= 2));
-      if (parts[i]) {   // the parts are those of consecutive blocks, as the joining kernel takes them
-        int c0 = 0;
-        while (split_at(units, blocks, c0 + 1) <= first) ++c0;
-        NEED(split_last(units, blocks, end[i]) - c0 + 1 == parts[i]);
+    NEED(at == slots && (slots == 0 || hi - lo <= 1));
+    std::vector<int> joined(batch * items);
+    for (int c = 0; c < workers; ++c)
+      if (joins[c].parts) {
+        const auto &s = seen[joins[c].b * items + joins[c].item];
+        ++joined[joins[c].b * items + joins[c].item];
+        NEED(s.front() == c && s.back() == c + joins[c].parts - 1);
+        for (size_t u = 1; u < s.size(); ++u) NEED(s[u] == s[u - 1] || s[u] == s[u - 1] + 1);   // nobody between has nothing
       }
-    }
+    for (size_t i = 0; i < seen.size(); ++i)
+      if (!seen[i].empty()) {
+        for (int c : seen[i]) NEED(c >= 0);
+        NEED(joined[i] == (seen[i].front() != seen[i].back()));
+      }
   }
-  // far: 2^31 - 1 tokens in each of 2^20 sequences
-  const long long units = (1LL << 20) * units_of(2147483647, 32) * 64;
-  NEED(units_of(2147483647, 32) == 1 << 26 && split_at(units, 296, 296) == units && split_at(units, 296, 0) == 0 && split_last(units, 296, units) == 295);
+  // far: 2^31 - 1 tokens in each of 2^20 sequences of 64 heads
+  const long long slots = (1LL << 20) * slots_of(2147483647, 16, 64);
+  NEED(units_of(2147483647, 16) == 1 << 27 && split_at(slots, 1184, 1184) == slots && split_at(slots, 1184, 0) == 0 && split_last(slots, 1184, slots) == 1183);
   puts("ok");
   return 0;
 }
 '''
 
 
-def test_dealing_of_units_to_blocks(tmp_path):
+def test_dealing_of_the_cache_to_warps(tmp_path):
     build_and_run(tmp_path, SPLIT)
