@@ -72,7 +72,15 @@ SB_HD void search_narrow(int &lo, int &hi, int k) {
 // in an earlier one, place 1 when it begins here and goes on.  A worker has at most one of each.
 constexpr int ITEM_COST = 1;
 
-SB_HD long long split_at(long long slots, int workers, int c) { return slots / workers * c + slots % workers * c / workers; }
+// Quotient of numbers from 0 on; 32 bits where they are enough (a 64-bit division is a routine of a hundred instructions).
+SB_HD long long quotient(long long a, long long b) {
+  return ((unsigned long long)(a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
+SB_HD long long split_at(long long slots, int workers, int c) {   // workers below 2^15: the rest's share fits 32 bits
+  const long long each = quotient(slots, workers);
+  return each * c + (unsigned)(slots - each * workers) * (unsigned)c / (unsigned)workers;
+}
 
 // The last worker that holds a slot before `end`, 0 < end <= slots.
 SB_HD int split_last(long long slots, int workers, long long end) {
@@ -87,12 +95,12 @@ SB_HD int split_last(long long slots, int workers, long long end) {
 
 // Workers that get work: none fewer than `least` slots, unless there are fewer in all.
 SB_HD int split_workers(long long slots, int workers, int least) {
-  const long long most = (slots + least - 1) / least;
+  const long long most = quotient(slots + least - 1, least);
   return most < 1 ? 1 : most < workers ? (int)most : workers;
 }
 
 // Units of a sequence of n tokens.
-SB_HD int units_of(int n, int unit) { return (int)(((long long)n + unit - 1) / unit); }
+SB_HD int units_of(int n, int unit) { return (int)(((unsigned)n + (unsigned)unit - 1u) / (unsigned)unit); }   // n below 2^31
 
 // Slots of all items of a sequence.
 SB_HD long long slots_of(int n, int unit, int items) { return n > 0 ? ((long long)units_of(n, unit) + ITEM_COST) * items : 0; }
@@ -107,8 +115,8 @@ struct Cursor {
 SB_HD void cursor_start(Cursor &c, long long offset, int unit) {
   c.units = units_of(c.len, unit);
   const long long per = (long long)c.units + ITEM_COST;
-  c.item = (int)(offset / per);
-  const long long o = offset % per;
+  c.item = (int)quotient(offset, per);
+  const long long o = offset - c.item * per;
   c.unit = o > ITEM_COST ? (int)(o - ITEM_COST) : 0;
   if (o < ITEM_COST) c.left -= ITEM_COST - o;
 }

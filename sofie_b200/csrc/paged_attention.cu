@@ -20,7 +20,7 @@ using namespace ptx;
 
 constexpr int PA_UNIT = 16;       // keys
 constexpr int PA_ROWS = 16;       // query heads of an item at most: the rows of one mma tile
-constexpr int PA_LEAST = 6;       // slots that are worth a worker of their own
+constexpr int PA_LEAST = 3;       // slots that are worth a worker of their own
 constexpr float PA_MARGIN = 16.f; // the reference maximum moves when a score is 2^16 above it: fp32 keeps its relative precision up there
 
 struct PagedAttnParams {
@@ -519,26 +519,44 @@ __global__ void __launch_bounds__(F32Cfg<DP, R>::THREADS) paged_fma_kernel(const
 constexpr int PJ_THREADS = 512, PJ_SLICES = PJ_THREADS / 32, PJ_FEW = 16;
 template <class T>
 __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const __grid_constant__ PagedAttnParams p, int workers, int dp) {
-  __shared__ int found[PJ_THREADS / 32 + 1];
-  __shared__ float red[PJ_SLICES][32], red_l[PJ_SLICES];
+  extern __shared__ __align__(16) int4 joins[];   // [workers]
+  __shared__ int found[PJ_THREADS / 32], s_first;
+  __shared__ float red[PJ_SLICES][32], red_l[PJ_SLICES], found_m[PJ_SLICES];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+#pragma unroll 4
+  for (int i = tid; i < workers; i += PJ_THREADS) joins[i] = p.joins[i];
+  __syncthreads();
   // ---- items of few parts: those of workers blockIdx.x, blockIdx.x + gridDim.x, ... ----
   for (int task = warp;; task += PJ_THREADS / 32) {
     const int w = blockIdx.x + task / p.rows * gridDim.x, r = task % p.rows;
     if (w >= workers) break;
-    const int4 j = p.joins[w];
+    const int4 j = joins[w];
     const int parts = j.z, key_head = j.y / p.parts_per_key, row0 = j.y % p.parts_per_key * PA_ROWS;
     if (parts < 2 || parts > PJ_FEW || row0 + r >= p.group) continue;
     auto place = [&](int i) { return ((long long)(w + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + r; };
     const float m = lane < parts ? p.part_m[place(lane)] : -INFINITY, l = lane < parts ? p.part_l[place(lane)] : 0.f;
+    float part[2][8];   // the first two parts come with the maxima
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (32 * k < dp) part[i][k] = p.part_o[place(i) * dp + lane + 32 * k];
     float M = m;
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float f = ex2(m - (M == -INFINITY ? 0.f : M));
     float L = l * f;
     for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     float acc[8] = {};
-    for (int i = 0; i < parts; ++i) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float g = __shfl_sync(0xffffffffu, f, i);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (32 * k < dp) acc[k] = fmaf(g, part[i][k], acc[k]);
+    }
+#pragma unroll 2
+    for (int i = 2; i < parts; ++i) {
       const float g = __shfl_sync(0xffffffffu, f, i);
       const float *src = p.part_o + place(i) * dp + lane;
 #pragma unroll
@@ -554,8 +572,8 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const __grid_con
   const int chunks = dp / 32, per_item = p.rows * chunks;
   int task = blockIdx.x, seen = 0;   // tasks of the items found so far
   for (int base = 0; base < workers; base += PJ_THREADS) {
-    const int4 j = base + tid < workers ? p.joins[base + tid] : make_int4(0, 0, 0, 0);
-    const uint32_t mask = __ballot_sync(0xffffffffu, j.z > PJ_FEW);
+    const bool many = base + tid < workers && joins[base + tid].z > PJ_FEW;
+    const uint32_t mask = __ballot_sync(0xffffffffu, many);
     if (lane == 0) found[warp] = __popc(mask);
     __syncthreads();
     int before = 0, all = 0;
@@ -563,42 +581,48 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const __grid_con
       if (w < warp) before += found[w];
       all += found[w];
     }
-    const int mine = j.z > PJ_FEW ? before + __popc(mask & ((1u << lane) - 1)) : -1;   // this thread's item among those of the round
-    __shared__ int4 s_item;
-    __shared__ int s_worker;
+    const int mine = many ? before + __popc(mask & ((1u << lane) - 1)) : -1;   // this thread's item among those of the round
     while (task < seen + all * per_item) {
       const int t = task - seen, item = t / per_item, r = t % per_item / chunks, d = t % chunks * 32 + lane;
-      if (mine == item) s_item = j, s_worker = base + tid;
+      if (mine == item) s_first = base + tid;
       __syncthreads();
-      const int4 it = s_item;
-      const int first = s_worker, parts = it.z;
-      const int key_head = it.y / p.parts_per_key, row0 = it.y % p.parts_per_key * PA_ROWS;
+      const int first = s_first;
+      const int4 it = joins[first];
+      const int parts = it.z, key_head = it.y / p.parts_per_key, row0 = it.y % p.parts_per_key * PA_ROWS;
       if (row0 + r < p.group) {
         auto place = [&](int i) { return ((long long)(first + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + r; };
-        float M = -INFINITY;
-        for (int i = lane; i < parts; i += 32) M = fmaxf(M, p.part_m[place(i)]);
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-        const float off = M == -INFINITY ? 0.f : M;
-        float L = 0.f, o = 0.f;
+        // each warp its slice of the parts, by the slice's own maximum
         const int per = (parts + PJ_SLICES - 1) / PJ_SLICES, i0 = min(parts, warp * per), i1 = min(parts, i0 + per);
+        float M = -INFINITY, L = 0.f, o = 0.f;
+        for (int at = i0; at < i1; at += 32) {
+          const int n = min(32, i1 - at);
+          const float m = lane < n ? p.part_m[place(at + lane)] : -INFINITY, l = lane < n ? p.part_l[place(at + lane)] : 0.f;
+          float top = fmaxf(m, M);
+          for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+          const float off = top == -INFINITY ? 0.f : top, again = ex2(M - off), f = ex2(m - off);
+          float sum = l * f;
+          for (int s = 16; s; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+          L = L * again + sum;
+          o *= again;
+          M = top;
 #pragma unroll 8
-        for (int i = i0; i < i1; ++i) {
-          const long long s = place(i);
-          const float f = ex2(p.part_m[s] - off);
-          L += p.part_l[s] * f;
-          o += p.part_o[s * dp + d] * f;
+          for (int i = 0; i < n; ++i) o = fmaf(__shfl_sync(0xffffffffu, f, i), p.part_o[place(at + i) * dp + d], o);
         }
         red[warp][lane] = o;
-        if (lane == 0) red_l[warp] = L;
+        if (lane == 0) red_l[warp] = L, found_m[warp] = M;
         __syncthreads();
         if (warp == 0) {
+          float top = -INFINITY;
+          for (int w = 0; w < PJ_SLICES; ++w) top = fmaxf(top, found_m[w]);
+          const float off = top == -INFINITY ? 0.f : top;
           o = L = 0.f;
           for (int w = 0; w < PJ_SLICES; ++w) {
-            o += red[w][lane];
-            L += red_l[w];
+            const float f = ex2(found_m[w] - off);
+            o = fmaf(f, red[w][lane], o);
+            L = fmaf(f, red_l[w], L);
           }
           if (d < p.dim)
-            from_f32(static_cast<T *>(p.y) + it.x * p.ldy + (long long)(key_head * p.group + row0 + r) * p.dim + d, M == -INFINITY ? 0.f : o / L);
+            from_f32(static_cast<T *>(p.y) + it.x * p.ldy + (long long)(key_head * p.group + row0 + r) * p.dim + d, top == -INFINITY ? 0.f : o / L);
         }
       }
       __syncthreads();
@@ -751,6 +775,7 @@ int sofie_b200_paged_attention_enqueue(sofie_b200_paged_attention_plan *plan, co
     const int64_t tasks = (int64_t)grid * warps * p.rows * (dp / 32);
     cfg.gridDim = dim3((unsigned)(tasks < ctx->sm_count ? tasks : ctx->sm_count));
     cfg.blockDim = dim3(PJ_THREADS);
+    cfg.dynamicSmemBytes = (size_t)grid * warps * sizeof(int4);   // below 48 KB: workers are what an SM keeps, 8 at most
     cfg.stream = ctx->stream;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
