@@ -189,23 +189,30 @@ class Context:
         packed, for PromptAttentionPlan.  cos, sin: fp32 [positions, rotary_dim / 2], absent = no rotation.  cu_seqlens: int32
         [batch + 1], the packed rows of each sequence; absent = one token per sequence.  Token rows may be column blocks of a
         wider tensor.  q_out may be q, k_out may be k."""
-        tokens, kv_heads, dim, ldk = _rows("k", k)
+        tokens, kv_heads, dim, ldk, pk = _rows("k", k)
         dtype = k.dtype
         if kv_heads != kv.kv_heads or dim != kv.head_dim or dtype is not kv.dtype:
             raise ValueError(f"kv_append: keys of {kv_heads} heads of {dim} {dtype}, cache of {kv.kv_heads} of {kv.head_dim} {kv.dtype}")
-        ldv = _same_rows("v", v, k)
-        ldko = _same_rows("k_out", k_out, k) if k_out is not None else 0
-        heads = ldq = ldqo = 0
+        n, h, e, ldv, pv = _rows("v", v)
+        if n != tokens or h != kv_heads or e != dim or v.dtype is not dtype:
+            raise ValueError(f"kv_append: values {tuple(v.shape)} {v.dtype} beside keys {tuple(k.shape)} {dtype}")
+        ldko = heads = ldq = ldqo = rotary = positions = 0
+        pko = pq = pqo = pcos = psin = pcu = None
+        if k_out is not None:
+            n, h, e, ldko, pko = _rows("k_out", k_out)
+            if n != tokens or h != kv_heads or e != dim or k_out.dtype is not dtype:
+                raise ValueError(f"kv_append: k_out {tuple(k_out.shape)} {k_out.dtype} beside keys {tuple(k.shape)} {dtype}")
         if q is not None:
             if q_out is None:
                 raise ValueError("kv_append: q needs q_out")
-            n, heads, qdim, ldq = _rows("q", q)
-            if n != tokens or qdim != dim or q.dtype is not dtype:
+            n, heads, e, ldq, pq = _rows("q", q)
+            m, h, f, ldqo, pqo = _rows("q_out", q_out)
+            if n != tokens or e != dim or q.dtype is not dtype:
                 raise ValueError("kv_append: q and k differ in tokens, head size or type")
-            ldqo = _same_rows("q_out", q_out, q)
+            if m != tokens or h != heads or f != dim or q_out.dtype is not dtype:
+                raise ValueError(f"kv_append: q_out {tuple(q_out.shape)} {q_out.dtype} beside queries {tuple(q.shape)} {dtype}")
         elif q_out is not None:
             raise ValueError("kv_append: q_out needs q")
-        rotary = positions = 0
         if cos is not None or sin is not None:
             if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or not (cos.is_contiguous() and sin.is_contiguous()):
                 raise ValueError("kv_append: cos and sin are two contiguous tensors of one shape [positions, rotary_dim / 2]")
@@ -213,12 +220,12 @@ class Context:
                 raise TypeError("kv_append: cos and sin are fp32")
             positions, rotary = cos.shape
             rotary *= 2
+            if rotary:
+                pcos, psin = _ptr(cos), _ptr(sin)
         if cu_seqlens is not None:
-            _offsets("cu_seqlens", cu_seqlens, kv.batch)
+            pcu = _offsets("cu_seqlens", cu_seqlens, kv.batch)
         d = L.KvAppendDesc(tokens, heads, kv_heads, dim, rotary, 1 if interleaved else 0, kv._dtype_code, positions, ldq, ldk, ldv, ldqo, ldko)
-        status = self._lib.sofie_b200_kv_append_enqueue(
-            self._h, C.byref(d), kv._ref, _ptr(cu_seqlens), _ptr(q), _ptr(k), _ptr(v), _ptr(cos) if rotary else None, _ptr(sin) if rotary else None,
-            _ptr(q_out), _ptr(k_out))
+        status = self._lib.sofie_b200_kv_append_enqueue(self._h, C.byref(d), kv._ref, pcu, pq, pk, pv, pcos, psin, pqo, pko)
         if status:
             L.check(status, "kv_append_enqueue")
 
@@ -244,7 +251,8 @@ class Context:
 
 
 def _rows(name, t):
-    """(tokens, heads, head size, token pitch) of a [tokens, heads, head_dim] tensor whose rows may be column blocks of wider ones."""
+    """(tokens, heads, head size, token pitch, address) of a [tokens, heads, head_dim] tensor on the GPU whose rows may be column
+    blocks of wider ones."""
     shape = t.shape
     if len(shape) != 3:
         raise ValueError(f"{name}: [tokens, heads, head_dim] is expected, not {tuple(shape)}")
@@ -252,19 +260,16 @@ def _rows(name, t):
     sn, sh, sd = t.stride()
     if (sd != 1 and d > 1) or (sh != d and h > 1):
         raise ValueError(f"{name}: the heads of a token must lie one behind another (strides {t.stride()})")
-    return n, h, d, sn if n > 1 else h * d
-
-
-def _same_rows(name, t, like):
-    """Token pitch of `t`, which has the shape and type of `like`."""
-    if t.shape != like.shape or t.dtype is not like.dtype:
-        raise ValueError(f"{name}: {tuple(like.shape)} {like.dtype} is expected, not {tuple(t.shape)} {t.dtype}")
-    return _rows(name, t)[3]
+    if not t.is_cuda:
+        raise ValueError("sofie_b200 operators take CUDA tensors; host data goes through run_host()")
+    return n, h, d, sn if n > 1 else h * d, t.data_ptr()
 
 
 def _offsets(name, t, batch):
+    """Address of an int32 tensor of batch + 1 row offsets on the GPU."""
     if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != batch + 1 or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous int32 tensor of batch + 1 = {batch + 1} row offsets is expected")
+    return _ptr(t)
 
 
 class PagedKV:
@@ -325,19 +330,21 @@ class PromptAttentionPlan:
     def enqueue(self, q, k, v, y, cu_seqlens, cu_seqlens_k=None) -> None:
         """q, y: [tokens, heads, head_dim]; k, v: [key tokens, kv_heads, head_dim], rows packed sequence behind sequence;
         cu_seqlens (and cu_seqlens_k, where keys have other lengths than queries): int32 [batch + 1] row offsets."""
-        n, h, d, ldq = _rows("q", q)
-        nk, hk, dk, ldk = _rows("k", k)
-        if (h, hk, d) != self._shape or dk != d or q.dtype is not self._dtype or k.dtype is not self._dtype:
-            raise ValueError(f"prompt attention: q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype} do not match the plan")
-        batch = cu_seqlens.shape[0] - 1
+        dtype = self._dtype
+        n, h, d, ldq, pq = _rows("q", q)
+        nk, hk, dk, ldk, pk = _rows("k", k)
+        nv, hv, dv, ldv, pv = _rows("v", v)
+        ny, hy, dy, ldy, py = _rows("y", y)
+        if (h, hk, d) != self._shape or dk != d or nv != nk or hv != hk or dv != d or ny != n or hy != h or dy != d:
+            raise ValueError(f"prompt attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, y {tuple(y.shape)} do not match the plan")
+        if q.dtype is not dtype or k.dtype is not dtype or v.dtype is not dtype or y.dtype is not dtype:
+            raise ValueError(f"prompt attention: {q.dtype}, {k.dtype}, {v.dtype}, {y.dtype} where the plan has {dtype}")
+        batch = cu_seqlens.numel() - 1
         if batch < 0:
             raise ValueError("cu_seqlens: batch + 1 row offsets are expected")
-        _offsets("cu_seqlens", cu_seqlens, batch)
-        if cu_seqlens_k is not None:
-            _offsets("cu_seqlens_k", cu_seqlens_k, batch)
-        status = self._lib.sofie_b200_prompt_attention_enqueue(
-            self._plan((ldq, ldk, _same_rows("v", v, k), _same_rows("y", y, q))), _ptr(q), _ptr(k), _ptr(v), _ptr(y), _ptr(cu_seqlens),
-            _ptr(cu_seqlens_k), batch, n, nk)
+        pcu = _offsets("cu_seqlens", cu_seqlens, batch)
+        pck = _offsets("cu_seqlens_k", cu_seqlens_k, batch) if cu_seqlens_k is not None else None
+        status = self._lib.sofie_b200_prompt_attention_enqueue(self._plan((ldq, ldk, ldv, ldy)), pq, pk, pv, py, pcu, pck, batch, n, nk)
         if status:
             L.check(status, "prompt_attention_enqueue")
 
@@ -370,6 +377,7 @@ class PagedAttentionPlan:
             self._workspace = torch.empty(size, dtype=torch.uint8, device=f"cuda:{ctx.device}")
             if ctx.stream is not None:   # freed memory must not be handed out again while the context's stream still uses it
                 self._workspace.record_stream(ctx.stream)
+        self._workspace_ptr = _ptr(self._workspace)
 
     def _plan(self, pitches):
         h = self._plans.get(pitches)
@@ -386,11 +394,15 @@ class PagedAttentionPlan:
 
     def enqueue(self, q, kv, y) -> None:
         """q, y: [batch, heads, head_dim]; kv: the PagedKV with the cache and its batch of sequences."""
-        n, h, d, ldq = _rows("q", q)
-        if (h, kv.kv_heads, d) != self._shape or kv.head_dim != d or q.dtype is not self._dtype or kv.dtype is not self._dtype or n != kv.batch:
+        dtype = self._dtype
+        n, h, d, ldq, pq = _rows("q", q)
+        ny, hy, dy, ldy, py = _rows("y", y)
+        if (h, kv.kv_heads, d) != self._shape or kv.head_dim != d or n != kv.batch or q.dtype is not dtype or kv.dtype is not dtype:
             raise ValueError(f"paged attention: q {tuple(q.shape)} {q.dtype} over {kv.batch} sequences of {kv.kv_heads} heads of {kv.head_dim} "
                              f"{kv.dtype} does not match the plan")
-        status = self._lib.sofie_b200_paged_attention_enqueue(self._plan((ldq, _same_rows("y", y, q))), _ptr(q), kv._ref, _ptr(y), _ptr(self._workspace))
+        if ny != n or hy != h or dy != d or y.dtype is not dtype:
+            raise ValueError(f"paged attention: y {tuple(y.shape)} {y.dtype} beside q {tuple(q.shape)} {dtype}")
+        status = self._lib.sofie_b200_paged_attention_enqueue(self._plan((ldq, ldy)), pq, kv._ref, py, self._workspace_ptr)
         if status:
             L.check(status, "paged_attention_enqueue")
 
@@ -398,7 +410,7 @@ class PagedAttentionPlan:
         for h in self._plans.values():
             self._lib.sofie_b200_paged_attention_plan_destroy(h)
         self._plans = {}
-        self._workspace = None
+        self._workspace = self._workspace_ptr = None
 
     def __del__(self):
         try:

@@ -128,16 +128,13 @@ def test_python_handles_refuse(b200_lib):
                 (k, k.transpose(0, 1).contiguous().transpose(0, 1), table, lens), (k, k, table, lens)):   # the last: not on a GPU
         with pytest.raises(ValueError):
             ops.PagedKV(*bad)
-    assert ops._rows("x", z(5, 12, 64)[:, 2:6]) == (5, 4, 64, 12 * 64)
-    assert ops._rows("x", z(1, 12, 64)[:, 2:6]) == (1, 4, 64, 4 * 64)
-    with pytest.raises(ValueError):
-        ops._rows("x", z(5, 4, 64).transpose(1, 2))
-    with pytest.raises(ValueError):
-        ops._rows("x", z(5, 8, 64)[:, ::2])
-    with pytest.raises(ValueError):
-        ops._rows("x", z(5, 64))
-    with pytest.raises(ValueError):
-        ops._offsets("cu", z(4, dt=torch.int32), 2)
+    for bad, text in ((z(5, 4, 64).transpose(1, 2), "one behind another"), (z(5, 8, 64)[:, ::2], "one behind another"), (z(5, 64), "is expected"),
+                      (z(5, 12, 64)[:, 2:6], "CUDA")):
+        with pytest.raises(ValueError, match=text):
+            ops._rows("x", bad)
+    for bad in (z(4, dt=torch.int32), z(3), z(3, 1, dt=torch.int32), z(6, dt=torch.int32)[::2], z(3, dt=torch.int32)):   # the last: not on a GPU
+        with pytest.raises(ValueError):
+            ops._offsets("cu", bad, 2)
 
 
 HOSTILE = r'''

@@ -546,4 +546,14 @@ def test_refusals_with_a_context(ctx):
     with pytest.raises(L.SofieB200Error, match="head size"):
         PromptAttentionPlan(ctx, 4, 2, 68, BF)
     prompt.enqueue(q[:0], k, k, q[:0], ints([0]))     # nothing to do is not an error
+    for kw in (dict(q=q), dict(q_out=q), dict(q=q, q_out=q[:1]), dict(cos=torch.zeros(4, 8, device=DEV)), dict(k_out=q),
+               dict(cos=torch.zeros(4, 8, device=DEV), sin=torch.zeros(4, 9, device=DEV))):
+        with pytest.raises(ValueError):
+            ctx.kv_append(k, k, kv, **kw)
+    with pytest.raises(ValueError):
+        ctx.kv_append(k, k[:1], kv)
+    with pytest.raises(ValueError):
+        ctx.kv_append(k, k, kv, ints([0, 2]))
+    with pytest.raises(TypeError):
+        ctx.kv_append(k, k, kv, cos=torch.zeros(40, 8, device=DEV, dtype=BF), sin=torch.zeros(40, 8, device=DEV, dtype=BF))
     ctx.sync()
