@@ -555,6 +555,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       const int n = (lim_hi + KEYS - 1) / KEYS, begin = first_turn(t, n, x);
       const bool mine = in_tile < per && query < t.queries;   // rows past the last query (and past per * group) hold anything
       const int lim = mine ? seen(p, t, query) : lim_hi;
+      const bool busy = __any_sync(0xffffffffu, mine);        // a warp without rows keeps step and computes nothing
       float m = -INFINITY, l = 0.f;   // reference maximum of the unscaled scores; sum of the weights
       // a tile's maximum: moves the reference maximum if it has to, and with it the sum and O
       auto raise = [&](float top, bool first) {
@@ -587,9 +588,11 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         const int base = (n - 1 - it) * KEYS;
         if (!(ok = warp_wait(bar_s + 8 * x, turns & 1, abort_flag))) break;
         tc_fence_after();
-        const int have = lim - base;   // keys of this tile that the row sees
+        const int have = lim - base, some = lim_hi - base;   // keys of this tile that the row sees; that any row sees (the product stops there)
         const bool masked = base + KEYS > lim_lo, first = it == begin;
-        if constexpr (Cfg::HOLD) {
+        if (!busy) {
+          if (Cfg::EARLY && lane == 0) mbar_arrive(bar_se + 8 * x);
+        } else if constexpr (Cfg::HOLD) {
           uint32_t r[KEYS];
           float *s = reinterpret_cast<float *>(r);
 #pragma unroll
@@ -655,11 +658,12 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             const float off = m == -INFINITY ? 0.f : -m * c;
             float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int k = 0; k < KEYS; k += 32) weigh(k, make_float2(off, off), sum);
+            for (int k = 0; k < KEYS; k += 32)
+              if (k < some) weigh(k, make_float2(off, off), sum);
             l += sum.x + sum.y;
           }
         } else {
-          // twice from tensor memory, 32 columns at a time: once for the maximum, once for the weights
+          // twice from tensor memory, 64 columns at a time: once for the maximum, once for the weights
           uint32_t r[32], other[32];
           float top = -INFINITY;
           auto take = [&](uint32_t *w, int at) {
@@ -675,14 +679,13 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             }
             top = fmaxf(top, fmaxf(x0, x1));
           };
-#pragma unroll
-          for (int k = 0; k < KEYS; k += 64) {
-            if (k == 0) tmem_ld_x32(t_s, r);
-            tmem_ld_wait();
+          const int end = some > KEYS - 64 ? KEYS : (some + 63) / 64 * 64;   // columns worth looking at
+#pragma unroll 1
+          for (int k = 0; k < end; k += 64) {
+            tmem_ld_x32(t_s + k, r);
             tmem_ld_x32(t_s + k + 32, other);
-            take(r, k);
             tmem_ld_wait();
-            if (k + 64 < KEYS) tmem_ld_x32(t_s + k + 64, r);
+            take(r, k);
             take(other, k + 32);
           }
           if (Cfg::EARLY && !first) {   // the previous product has left P and O
@@ -690,7 +693,6 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             tc_fence_after();
           }
           raise(top, first);
-          tmem_ld_x32(t_s, r);
           const float off = m == -INFINITY ? 0.f : -m * c;
           const float2 off2 = make_float2(off, off);
           float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
@@ -714,19 +716,17 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             }
             tmem_st_x16(t_p + at / 2, w);
           };
-#pragma unroll
-          for (int k = 0; k < KEYS; k += 64) {
-            tmem_ld_wait();
+#pragma unroll 1
+          for (int k = 0; k < end; k += 64) {
+            tmem_ld_x32(t_s + k, r);
             tmem_ld_x32(t_s + k + 32, other);
-            weigh(r, k);
             tmem_ld_wait();
-            if (k + 64 < KEYS) {
-              tmem_ld_x32(t_s + k + 64, r);
-            } else if (Cfg::EARLY) {   // the scores are read
+            if (Cfg::EARLY && k + 64 >= end) {   // the scores are read
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(bar_se + 8 * x);
             }
+            weigh(r, k);
             weigh(other, k + 32);
           }
           l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
@@ -742,6 +742,10 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         ++results;
         tc_fence_after();
         plain = unclean[i & 3] == i + 1;
+      }
+      if (!busy) {
+        if (begin < n && lane == 0) mbar_arrive(bar_oe + 8 * x);
+        continue;
       }
       const float inv = 1.f / l;
       const bool none = begin == n || lim <= 0;
@@ -902,13 +906,14 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           if (Cfg::EARLY && it + 1 < n && !(ok = scores(0, it + 1))) break;
           if (!(ok = warp_wait(bar_full + 8 * vs, vph, abort_flag))) break;
           if (base + KEYS > visible) {
-            // Values past the last key that anybody here sees belong to others and may hold anything: zeros in their place, since
-            // the tensor cores multiply every value by every row's weight and 0 * NaN is NaN.  Values on the diagonal are hidden
+            // The product takes 16 keys at a time and stops after the last one that anybody here sees.  Values past that key belong
+            // to others and may hold anything: zeros in their place, since the tensor cores multiply every value by every row's
+            // weight and 0 * NaN is NaN.  Values on the diagonal are hidden
             // from some rows only: if one is not finite, the rows are summed up the plain way at the end.
             uint8_t *v = gen + QS * Cfg::Q + vs * Cfg::TILE;
             constexpr int PIECES = 8 * Cfg::PANELS;   // 16-byte pieces of a key's values
             const int none = max(0, min(KEYS, lim_hi - base)), some = max(0, min(none, lim_lo - base));
-            for (int k = none * PIECES + lane; k < KEYS * PIECES; k += 32) {
+            for (int k = none * PIECES + lane; k < (none + 15) / 16 * 16 * PIECES; k += 32) {
               const int key = k / PIECES, piece = k % PIECES;
               *reinterpret_cast<uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
@@ -923,6 +928,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             __syncwarp();
           }
           const uint32_t v_lo = mnmajor | (ring + vs * (Cfg::TILE >> 4));
+          const int last_key = (int)uniform(lim_hi - base);
 #pragma unroll
           for (int x = 0; x < TILES; ++x) {
             if (it >= begin[x]) {
@@ -932,8 +938,8 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               tc_fence_after();
 #pragma unroll
               for (int kk = 0; kk < KEYS / 16; ++kk)   // 16 keys: 8 columns of P, 16 rows of V
-                umma_ts(leader, tm + Cfg::O_COL + x * Cfg::STEP, tm + Cfg::P_COL + x * Cfg::STEP + 8 * kk, desc_hi | (v_lo + 128 * kk), idesc_o,
-                        kk != 0 ? 1u : more);
+                umma_ts(16 * kk < last_key ? leader : 0u, tm + Cfg::O_COL + x * Cfg::STEP, tm + Cfg::P_COL + x * Cfg::STEP + 8 * kk,
+                        desc_hi | (v_lo + 128 * kk), idesc_o, kk != 0 ? 1u : more);
               ++weighed[x];
               if (Cfg::EARLY) commit_if(leader, bar_pv + 8 * x);
             }
