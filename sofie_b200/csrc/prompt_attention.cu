@@ -347,33 +347,46 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t *r) {
       "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// The loads have arrived; nothing that uses their registers moves above this.
+template <int N>
+__device__ __forceinline__ void tmem_loaded(uint32_t (&r)[N]) {
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A block works on TILES tiles of 128 rows against the same keys and values.  What sets the sizes is the way from L2: a tile of keys
-// and values takes about 3000 cycles from request to arrival and an SM sustains about 48 bytes per cycle, while the tensor cores
-// would finish 128 rows x 128 keys of head size 128 (64 KB of keys and values) in 1024 cycles.  So at that head size two tiles of rows
-// share every load (32 bytes per cycle at full rate) and five tiles of keys or values are in flight; at head size 64 half the bytes
-// are needed per score, and two blocks of one tile share an SM instead.
+// A block works on TILES tiles of 128 rows against the same keys and values.  What sets the sizes:
+//  - The way from L2: a tile of keys and values takes about 3000 cycles from request to arrival and an SM sustains about 48 bytes per
+//    cycle, while the tensor cores would finish 128 rows x 128 keys of head size 128 (64 KB of keys and values) in 1024 cycles (512 for
+//    each product, measured alone).  So at that head size two tiles of rows share every load (32 bytes per cycle at full rate) and
+//    160 KB are in flight; one tile a block, two blocks an SM, with 64 KB in flight each, took 964 us where this takes 495 (a prompt
+//    of 8192 tokens, 32 heads over 8).  At head size 64 half the bytes are needed per score, and two blocks of one tile share an SM.
+//  - Tensor memory, 512 columns.  EARLY: the weights have columns of their own, and the scores of the next tile of keys are computed
+//    while this one's are weighed.  At head size 128 two results leave room for that with 64 keys a tile only, where the first product
+//    is bound by shared memory (533 us), or 80 keys (678 us, too many registers); there the weights lie over the scores, 128 keys a tile.
+//  - Exponentials: the special-function unit does 16 a cycle and SM, 1024 cycles for 128 x 128 scores, as long as both products.  Taking
+//    1/8 to 1/2 of them on the FMA pipes (a polynomial of degree 4) made every case slower: a warp is alone on its scheduler's special
+//    unit most of the time, and it is the length of its own chain that counts.
 template <int DP>
 struct UmmaCfg;
 template <>
-struct UmmaCfg<64> {
-  static constexpr int TILES = 1, KEYS = 128, BLOCKS = 2, STAGES = 4, QS = 2, COLS = 256;
-  static constexpr int S_COL = 0, O_COL = 128, P_COL = 192, STEP = 0;
+struct UmmaCfg<64> {   // 128 keys a tile, scores read twice from tensor memory: 540 us for 32 full sequences of 2048 tokens, this 457
+  static constexpr int TILES = 1, KEYS = 64, BLOCKS = 2, STAGES = 9, QS = 2, COLS = 256;
+  static constexpr int S_COL = 0, O_COL = 128, P_COL = 64, STEP = 0;
   static constexpr bool EARLY = true;    // the weights have columns of their own: the next scores are computed meanwhile
-  static constexpr bool HOLD = false;    // a thread holds its whole row of scores in registers
 };
 template <>
 struct UmmaCfg<128> {
   static constexpr int TILES = 2, KEYS = 128, BLOCKS = 1, STAGES = 5, QS = 1, COLS = 512;
   static constexpr int S_COL = 0, O_COL = 128, P_COL = 0, STEP = 256;
-  static constexpr bool EARLY = false, HOLD = true;
+  static constexpr bool EARLY = false;
 };
 template <>
 struct UmmaCfg<256> {
   static constexpr int TILES = 1, KEYS = 64, BLOCKS = 1, STAGES = 5, QS = 1, COLS = 512;
   static constexpr int S_COL = 0, O_COL = 256, P_COL = 64, STEP = 0;
-  static constexpr bool EARLY = true, HOLD = true;
+  static constexpr bool EARLY = true;
 };
 template <int DP>
 struct UmmaSize : UmmaCfg<DP> {
@@ -572,7 +585,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         for (int d = 0; d < DP; d += 16) {
           uint32_t o[16];
           tmem_ld_x16(t_o + d, o);
-          tmem_ld_wait();
+          tmem_loaded(o);
 #pragma unroll
           for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
           tmem_st_x16(t_o + d, o);
@@ -592,12 +605,14 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         const bool masked = base + KEYS > lim_lo, first = it == begin;
         if (!busy) {
           if (Cfg::EARLY && lane == 0) mbar_arrive(bar_se + 8 * x);
-        } else if constexpr (Cfg::HOLD) {
+          // in step with the others: two turns ahead, its word would stand for one that is still at work
+          if (Cfg::EARLY && !first && !(ok = warp_wait(bar_pv + 8 * x, (turns - 1) & 1, abort_flag))) break;
+        } else {
           uint32_t r[KEYS];
-          float *s = reinterpret_cast<float *>(r);
 #pragma unroll
           for (int k = 0; k < KEYS; k += 32) tmem_ld_x32(t_s + k, r + k);
-          tmem_ld_wait();
+          tmem_loaded(r);
+          float *s = reinterpret_cast<float *>(r);
           if (Cfg::EARLY) {
             tc_fence_before();
             __syncwarp();
@@ -662,74 +677,6 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               if (k < some) weigh(k, make_float2(off, off), sum);
             l += sum.x + sum.y;
           }
-        } else {
-          // twice from tensor memory, 64 columns at a time: once for the maximum, once for the weights
-          uint32_t r[32], other[32];
-          float top = -INFINITY;
-          auto take = [&](uint32_t *w, int at) {
-            float *s = reinterpret_cast<float *>(w);
-            if (masked)
-#pragma unroll
-              for (int k = 0; k < 32; ++k) s[k] = at + k < have ? s[k] : -INFINITY;
-            float x0 = s[0], x1 = s[1];
-#pragma unroll
-            for (int k = 2; k < 32; k += 2) {
-              x0 = fmaxf(x0, s[k]);
-              x1 = fmaxf(x1, s[k + 1]);
-            }
-            top = fmaxf(top, fmaxf(x0, x1));
-          };
-          const int end = some > KEYS - 64 ? KEYS : (some + 63) / 64 * 64;   // columns worth looking at
-#pragma unroll 1
-          for (int k = 0; k < end; k += 64) {
-            tmem_ld_x32(t_s + k, r);
-            tmem_ld_x32(t_s + k + 32, other);
-            tmem_ld_wait();
-            take(r, k);
-            take(other, k + 32);
-          }
-          if (Cfg::EARLY && !first) {   // the previous product has left P and O
-            if (!(ok = warp_wait(bar_pv + 8 * x, (turns - 1) & 1, abort_flag))) break;
-            tc_fence_after();
-          }
-          raise(top, first);
-          const float off = m == -INFINITY ? 0.f : -m * c;
-          const float2 off2 = make_float2(off, off);
-          float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
-          auto weigh = [&](const uint32_t *from, int at) {
-            const float *s = reinterpret_cast<const float *>(from);
-            uint32_t w[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float2 e = make_float2(s[2 * k], s[2 * k + 1]);
-              if (masked) {
-                e.x = at + 2 * k < have ? e.x : -INFINITY;
-                e.y = at + 2 * k + 1 < have ? e.y : -INFINITY;
-              }
-              e = __ffma2_rn(e, c2, off2);
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-              if (k & 1) sum1 = __fadd2_rn(sum1, e);
-              else sum0 = __fadd2_rn(sum0, e);
-              const __nv_bfloat162 h = __floats2bfloat162_rn(e.x, e.y);
-              w[k] = *reinterpret_cast<const uint32_t *>(&h);
-            }
-            tmem_st_x16(t_p + at / 2, w);
-          };
-#pragma unroll 1
-          for (int k = 0; k < end; k += 64) {
-            tmem_ld_x32(t_s + k, r);
-            tmem_ld_x32(t_s + k + 32, other);
-            tmem_ld_wait();
-            if (Cfg::EARLY && k + 64 >= end) {   // the scores are read
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar_se + 8 * x);
-            }
-            weigh(r, k);
-            weigh(other, k + 32);
-          }
-          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
         }
         hand_over();
       }
@@ -755,7 +702,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         uint32_t o[32];
         if (begin < n) {
           tmem_ld_x32(t_o + d, o);
-          tmem_ld_wait();
+          tmem_loaded(o);
           if (d + 32 == DP) {   // the next tile's products may begin
             tc_fence_before();
             __syncwarp();

@@ -262,6 +262,23 @@ def test_prompt_rows_far_from_the_maximum(ctx):
             ref.close(y, *ref.prompt(q, k, v, [0, n], [0, n], causal))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("heads,kvh,dim,n,std", [(5, 1, 8, 260, 1.5), (1, 1, 64, 520, 6.0), (4, 1, 64, 300, 6.0), (1, 1, 128, 520, 6.0), (4, 1, 128, 520, 6.0),
+                                                 (1, 1, 256, 520, 6.0), (3, 1, 80, 300, 5.0)])
+def test_prompt_maximum_moves_late(ctx, heads, kvh, dim, n, std, dtype):
+    """Peaked scores, and a last tile of keys of which a row sees few: the running maximum moves far in later tiles, in tiles of rows
+    whose last warps hold no rows."""
+    from sofie_b200.ops import PromptAttentionPlan
+    for seed in range(4):
+        g = gen_of(seed)
+        q, k, v = normal(g, (n, heads, dim), dtype, std), normal(g, (n, kvh, dim), dtype), normal(g, (n, kvh, dim), dtype)
+        for causal in (True, False):
+            y = torch.zeros_like(q)
+            PromptAttentionPlan(ctx, heads, kvh, dim, dtype, causal=causal).enqueue(q, k, v, y, ints([0, n]))
+            ctx.sync()
+            ref.close(y, *ref.prompt(q, k, v, [0, n], [0, n], causal), f"seed {seed}, causal {causal}")
+
+
 def test_prompt_bad_offsets_are_left_out(ctx):
     from sofie_b200.ops import PromptAttentionPlan
     for dtype in (BF, F32):
