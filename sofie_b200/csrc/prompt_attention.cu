@@ -120,24 +120,29 @@ __device__ __forceinline__ int seen(const PromptParams &p, const PromptTile &t, 
 }
 
 // ---- fp32 on the CUDA cores --------------------------------------------------------------------------------------------------------
-// A block of four warps computes 32 rows against tiles of 64 keys.  A thread has 4 rows x 4 keys of the scores and 4 rows x DP / 16
-// dimensions of the result, so that a 16-byte read from shared memory feeds 16 FMAs and the FMA pipes are what bounds it.  The next
-// keys arrive while this tile's values are weighed, the next values while the next scores are computed (cp.async, one place each).
-constexpr int PF_ROWS = 32, PF_KEYS = 64, PF_THREADS = 128;
+// A block computes 32 rows; each of its teams of four warps takes every TEAMS-th tile of 64 keys, and the teams' sums are joined at the end.
+// (Few blocks are long chains of tiles on few warps otherwise: 770 queries of 8 heads over 1770 keys take 80 us with one team, 71 us with
+// two; prompts of 2048 tokens 31 TFLOP/s, 0.42 of the FMA pipes, with either.  Above head size 128 a second team's tiles do not fit.)
+// A thread has 4 rows x 4 keys of the scores and 4 rows x DP / 16 dimensions of the result, so that a 16-byte read from shared memory
+// feeds 16 FMAs and the FMA pipes are what bounds it.  The next keys arrive while this tile's values are weighed, the next values while
+// the next scores are computed (cp.async, one place each).
+constexpr int PF_ROWS = 32, PF_KEYS = 64, PF_TEAM = 128;
 template <int DP>
 struct FmaCfg {
+  static constexpr int TEAMS = DP <= 128 ? 2 : 1, THREADS = TEAMS * PF_TEAM;
   static constexpr int Q = PF_ROWS * DP * 4, TILE = PF_KEYS * DP * 4, P = PF_KEYS * PF_ROWS * 4;
-  static constexpr int SMEM = Q + 2 * TILE + P + 4 * (RUNS + 1);
+  static constexpr int SMEM = Q + TEAMS * (2 * TILE + P) + 4 * (RUNS + 1);
 };
 
 template <int DP>
-__global__ void __launch_bounds__(PF_THREADS) prompt_fma_kernel(const __grid_constant__ PromptParams p, int parts) {
+__global__ void __launch_bounds__(FmaCfg<DP>::THREADS) prompt_fma_kernel(const __grid_constant__ PromptParams p, int parts) {
   using Cfg = FmaCfg<DP>;
   constexpr int CH = DP / 4, PIECES = DP / 64;   // 16-byte pieces of a row; of the result per thread and row
   extern __shared__ __align__(128) uint8_t smem[];
-  float4 *sq = reinterpret_cast<float4 *>(smem), *sk = sq + Cfg::Q / 16, *sv = sk + Cfg::TILE / 16, *sp = sv + Cfg::TILE / 16;
-  int *table = reinterpret_cast<int *>(smem + Cfg::Q + 2 * Cfg::TILE + Cfg::P);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int team = threadIdx.x / PF_TEAM, tid = threadIdx.x % PF_TEAM, warp = tid >> 5, lane = tid & 31;
+  float4 *sq = reinterpret_cast<float4 *>(smem), *sk = sq + (Cfg::Q + team * (2 * Cfg::TILE + Cfg::P)) / 16, *sv = sk + Cfg::TILE / 16, *sp = sv + Cfg::TILE / 16;
+  int *table = reinterpret_cast<int *>(smem + Cfg::Q + Cfg::TEAMS * (2 * Cfg::TILE + Cfg::P));
+  auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(PF_TEAM) : "memory"); };   // the team
   count_tiles(p, table);
   const int work = blockIdx.x / parts, part = blockIdx.x % parts, kh = work % p.kv_heads;   // a group of more than 32 heads is several parts
   const PromptTile t = find_tile(p, table, work / p.kv_heads);
@@ -152,21 +157,25 @@ __global__ void __launch_bounds__(PF_THREADS) prompt_fma_kernel(const __grid_con
 
   auto load_tile = [&](uint32_t dst, const float *src, long long pitch, int base, bool swizzle) {
 #pragma unroll 4
-    for (int i = tid; i < PF_KEYS * CH; i += PF_THREADS) {
+    for (int i = tid; i < PF_KEYS * CH; i += PF_TEAM) {
       const int r = i / CH, c = i % CH;
       const bool there = base + r < lim_hi && c * 4 < p.dim;
       cp_async_16(dst + (r * CH + (swizzle ? c ^ (r & 7) : c)) * 16, src + (there ? (base + r) * pitch + c * 4 : 0), there);
     }
   };
-  for (int i = tid; i < PF_ROWS * CH; i += PF_THREADS) {
+  const int begin = n - 1 - team;   // this team's tiles: begin, begin - TEAMS, ...
+  for (int i = threadIdx.x; i < PF_ROWS * CH; i += Cfg::THREADS) {
     const int r = i / CH, c = i % CH, query = r / heads, h = r - query * heads;
     const bool there = query < t.queries && c * 4 < p.dim;
     cp_async_16(a_q + i * 16, q + (there ? query * p.ldq + (long long)h * p.dim + c * 4 : 0), there);
   }
-  if (n > 0) load_tile(a_k, k, p.ldk, (n - 1) * PF_KEYS, true);
   cp_async_commit();
-  if (n > 0) load_tile(a_v, v, p.ldv, (n - 1) * PF_KEYS, false);
+  if (begin >= 0) load_tile(a_k, k, p.ldk, begin * PF_KEYS, true);
   cp_async_commit();
+  if (begin >= 0) load_tile(a_v, v, p.ldv, begin * PF_KEYS, false);
+  cp_async_commit();
+  cp_async_wait<2>();
+  __syncthreads();   // the queries, which both teams brought
 
   const int rg = warp * 2 + (lane >> 4), g = lane & 15;   // rows 4 rg .. 4 rg + 3; keys g + 16 j; pieces g + 16 j of the result
   int lim[4];
@@ -182,11 +191,11 @@ __global__ void __launch_bounds__(PF_THREADS) prompt_fma_kernel(const __grid_con
     for (int j = 0; j < PIECES; ++j) acc[r][j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 
-  for (int it = n - 1; it >= 0; --it) {
+  for (int it = begin; it >= 0; it -= Cfg::TEAMS) {
     const int base = it * PF_KEYS;
     const bool masked = base + PF_KEYS > lim_lo;
     cp_async_wait<1>();   // the keys
-    __syncthreads();
+    meet();
     float s[4][4] = {};
 #pragma unroll 2
     for (int c = 0; c < CH; ++c) {
@@ -200,8 +209,8 @@ __global__ void __launch_bounds__(PF_THREADS) prompt_fma_kernel(const __grid_con
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[r][j] = fmaf(a[r].x, b[j].x, fmaf(a[r].y, b[j].y, fmaf(a[r].z, b[j].z, fmaf(a[r].w, b[j].w, s[r][j]))));
     }
-    __syncthreads();   // the keys are read
-    if (it > 0) load_tile(a_k, k, p.ldk, base - PF_KEYS, true);
+    meet();   // the keys are read
+    if (it >= Cfg::TEAMS) load_tile(a_k, k, p.ldk, base - Cfg::TEAMS * PF_KEYS, true);
     cp_async_commit();
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -234,7 +243,7 @@ __global__ void __launch_bounds__(PF_THREADS) prompt_fma_kernel(const __grid_con
       sp[key * (PF_ROWS / 4) + (rg ^ (key & 7))] = make_float4(s[0][j], s[1][j], s[2][j], s[3][j]);
     }
     cp_async_wait<1>();   // the values
-    __syncthreads();
+    meet();
     if (!masked) {
 #pragma unroll 4
       for (int key = 0; key < PF_KEYS; ++key) {
@@ -271,11 +280,37 @@ __global__ void __launch_bounds__(PF_THREADS) prompt_fma_kernel(const __grid_con
         }
       }
     }
-    __syncthreads();   // values and weights are read
-    if (it > 0) load_tile(a_v, v, p.ldv, base - PF_KEYS, false);
+    meet();   // values and weights are read
+    if (it >= Cfg::TEAMS) load_tile(a_v, v, p.ldv, base - Cfg::TEAMS * PF_KEYS, false);
     cp_async_commit();
   }
   cp_async_wait<0>();
+  if constexpr (Cfg::TEAMS == 2) {   // the second team's sums onto the first one's, thread by thread
+    float4 *sum = reinterpret_cast<float4 *>(smem + Cfg::Q + (2 * Cfg::TILE + Cfg::P));   // the second team's keys, which are read
+    if (team == 1) {
+      meet();
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        sum[(r * (PIECES + 1)) * PF_TEAM + tid] = make_float4(m[r], l[r], 0.f, 0.f);
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) sum[(r * (PIECES + 1) + 1 + j) * PF_TEAM + tid] = acc[r][j];
+      }
+    }
+    __syncthreads();
+    if (team == 1) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float4 ml = sum[(r * (PIECES + 1)) * PF_TEAM + tid];
+      const float top = fmaxf(m[r], ml.x), off = top == -INFINITY ? 0.f : top, f = ex2(m[r] - off), g2 = ex2(ml.x - off);
+      m[r] = top;
+      l[r] = l[r] * f + ml.y * g2;
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) {
+        const float4 x = sum[(r * (PIECES + 1) + 1 + j) * PF_TEAM + tid];
+        acc[r][j] = make_float4(acc[r][j].x * f + x.x * g2, acc[r][j].y * f + x.y * g2, acc[r][j].z * f + x.z * g2, acc[r][j].w * f + x.w * g2);
+      }
+    }
+  }
 
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -975,7 +1010,7 @@ static int launch_fma(sofie_b200_ctx *ctx, PromptParams p) {
   if (grid > 0x7fffffffLL) return fail(SOFIE_B200_ERR_TOO_LARGE, "prompt_attention_enqueue: %lld queries of %d heads", p.q_rows, p.heads);
   if (!p.k_rows) p.k = p.v = p.q;   // nothing is read, but the address a copy of no bytes is given should exist
   SB_CUDA(cudaFuncSetAttribute(prompt_fma_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, FmaCfg<DP>::SMEM));   // per device
-  prompt_fma_kernel<DP><<<(unsigned)grid, PF_THREADS, FmaCfg<DP>::SMEM, ctx->stream>>>(p, parts);
+  prompt_fma_kernel<DP><<<(unsigned)grid, FmaCfg<DP>::THREADS, FmaCfg<DP>::SMEM, ctx->stream>>>(p, parts);
   SB_CUDA(cudaGetLastError());
   ctx->launches++;
   return 0;
