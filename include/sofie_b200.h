@@ -455,7 +455,8 @@ typedef struct sofie_b200_kv_append_desc {
 /* q [tokens, heads, head_dim] -> q_out, k and v [tokens, kv_heads, head_dim] -> the cache, and the rotated keys -> k_out too when
  * it is not NULL (what sofie_b200_prompt_attention_enqueue reads).  cos, sin: F32 [max_position, rotary_dim / 2].  q_out may be q and
  * k_out may be k (the same pointer and pitch); otherwise outputs overlap nothing.  cu_seqlens NULL: one token per sequence
- * (tokens == batch), where seq_lens[b] = 0 marks a padding row that is skipped.  No two tokens of a call share a slot of the cache. */
+ * (tokens == batch), where seq_lens[b] = 0 marks a padding row that is skipped.  No two tokens of a call share a slot of the cache.
+ * Sequences may share pages (a common prefix) as long as none is appended to in one. */
 int sofie_b200_kv_append_enqueue(sofie_b200_ctx *ctx, const sofie_b200_kv_append_desc *desc, const sofie_b200_paged_kv *kv,
                                  const int32_t *cu_seqlens, const void *q, const void *k, const void *v, const float *cos,
                                  const float *sin, void *q_out, void *k_out);
@@ -464,7 +465,8 @@ int sofie_b200_kv_append_enqueue(sofie_b200_ctx *ctx, const sofie_b200_kv_append
  * sequence -- all lk of them, or with causal = 1 those with j <= i + lk - lq (the last query sees the last key; lk > lq: a prompt
  * continued after lk - lq keys).  A query that sees no key gets zeros.  Keys and values that a query does not see have no
  * influence on it, whatever they hold (NaN and infinities included).
- * head_dim: a multiple of 8 up to 256; heads / kv_heads up to 64; token pitches multiples of 8 elements; tensors 16-byte aligned. */
+ * head_dim: a multiple of 8 up to 256; heads / kv_heads up to 64; token pitches multiples of 8 elements; tensors 16-byte aligned; up to
+ * 2^27 query and key rows. */
 typedef struct sofie_b200_prompt_attention_desc {
   int32_t heads, kv_heads, head_dim;
   int32_t dtype;                 /* F32 or BF16 */
@@ -476,8 +478,9 @@ typedef struct sofie_b200_prompt_attention_plan sofie_b200_prompt_attention_plan
 int sofie_b200_prompt_attention_plan_create(sofie_b200_ctx *ctx, const sofie_b200_prompt_attention_desc *desc,
                                             sofie_b200_prompt_attention_plan **out);
 int sofie_b200_prompt_attention_plan_destroy(sofie_b200_prompt_attention_plan *plan);
+/* "umma" (bf16, tensor cores) or "fma" (F32, CUDA cores) */
 const char *sofie_b200_prompt_attention_plan_kernel(const sofie_b200_prompt_attention_plan *plan);
-/* q, y: [q_tokens, heads, head_dim]; k, v: [k_tokens, kv_heads, head_dim].  cu_seqlens_k NULL = cu_seqlens_q. */
+/* q, y: [q_tokens, heads, head_dim]; k, v: [k_tokens, kv_heads, head_dim].  cu_seqlens_k NULL = cu_seqlens_q.  y overlaps no input. */
 int sofie_b200_prompt_attention_enqueue(sofie_b200_prompt_attention_plan *plan, const void *q, const void *k, const void *v, void *y,
                                         const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int64_t batch, int64_t q_tokens,
                                         int64_t k_tokens);
@@ -496,12 +499,13 @@ typedef struct sofie_b200_paged_attention_plan sofie_b200_paged_attention_plan;
 int sofie_b200_paged_attention_plan_create(sofie_b200_ctx *ctx, const sofie_b200_paged_attention_desc *desc,
                                            sofie_b200_paged_attention_plan **out);
 int sofie_b200_paged_attention_plan_destroy(sofie_b200_paged_attention_plan *plan);
+/* "mma" (bf16, tensor cores) or "fma" (F32, CUDA cores) */
 const char *sofie_b200_paged_attention_plan_kernel(const sofie_b200_paged_attention_plan *plan);
 /* Bytes of 256-byte aligned caller scratch for the parts of split sequences; depends on the plan alone, not on the batch or its
  * lengths.  Its contents need no preparation and mean nothing between calls.  Calls that may run at the same time (two streams,
  * two captured graphs replayed side by side) need a workspace each. */
 int64_t sofie_b200_paged_attention_workspace_bytes(const sofie_b200_paged_attention_plan *plan);
-/* q, y: [batch, heads, head_dim] (batch = kv->batch). */
+/* q, y: [batch, heads, head_dim] (batch = kv->batch).  y overlaps no input. */
 int sofie_b200_paged_attention_enqueue(sofie_b200_paged_attention_plan *plan, const void *q, const sofie_b200_paged_kv *kv, void *y,
                                        void *workspace);
 

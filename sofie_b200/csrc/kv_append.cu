@@ -283,7 +283,7 @@ static void launch_append(sofie_b200_ctx *ctx, const AppendParams &p) {
   // Few tokens: a block each, for the shortest way (120 tokens of 32 + 2 x 8 heads of 128: as long as an empty launch either way).  From
   // four for every SM on: two warps each, four tokens to a block; of 10,832 tokens a block takes 101 us, four warps 70, two 63, one 68.
   if (p.tokens < ctx->sm_count * 4) kv_append_kernel<T, V, 256><<<(unsigned)p.tokens, 256, 0, ctx->stream>>>(p);
-  else kv_append_kernel<T, V, 64><<<(unsigned)((p.tokens + 3) / 4), 256, 0, ctx->stream>>>(p);
+  else kv_append_kernel<T, V, 64><<<(unsigned)p.tokens / 4 + (p.tokens % 4 != 0), 256, 0, ctx->stream>>>(p);
 }
 template <class T>
 static void launch_append(sofie_b200_ctx *ctx, const AppendParams &p, int v) {

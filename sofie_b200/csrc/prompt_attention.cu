@@ -460,32 +460,23 @@ __device__ __forceinline__ bool block_given(uint32_t answer, uint32_t &index) {
   return given != 0;
 }
 
-// The plain sum for one row, from global memory.  Taken when values that some rows of a tile do not see hold NaN or infinities: the
-// tensor cores multiply every value by every row's weight, and 0 * NaN would reach rows it must not reach.
-__device__ __noinline__ void plain_row(const PromptParams &p, long long q_row, int head, int k0, int n) {
-  typedef __nv_bfloat16 T;
-  const T *q = static_cast<const T *>(p.q) + q_row * p.ldq + (long long)head * p.dim;
-  T *y = static_cast<T *>(p.y) + q_row * p.ldy + (long long)head * p.dim;
-  const int kh = head / p.group;
-  auto score = [&](int j) {
-    const T *k = static_cast<const T *>(p.k) + (long long)(k0 + j) * p.ldk + (long long)kh * p.dim;
-    float s = 0.f;
-    for (int d = 0; d < p.dim; ++d) s = fmaf(to_f32(q[d]), to_f32(k[d]), s);
-    return s * p.scale_log2e;
-  };
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < n; ++j) m = fmaxf(m, score(j));
-  if (m == -INFINITY) m = 0.f;
-  for (int d0 = 0; d0 < p.dim; d0 += 8) {
-    float acc[8] = {};
-    l = 0.f;
-    for (int j = 0; j < n; ++j) {
-      const float e = ex2(score(j) - m);
-      const T *v = static_cast<const T *>(p.v) + (long long)(k0 + j) * p.ldv + (long long)kh * p.dim + d0;
-      l += e;
-      for (int d = 0; d < 8; ++d) acc[d] = fmaf(e, to_f32(v[d]), acc[d]);
+// The result of a row += the NaN and infinities among the values of the sequence's keys [j0, j1), which the product went without.
+__device__ __noinline__ void add_nonfinite(const PromptParams &p, long long q_row, int head, int k0, int j0, int j1) {
+  __nv_bfloat16 *y = static_cast<__nv_bfloat16 *>(p.y) + q_row * p.ldy + (long long)head * p.dim;
+  const __nv_bfloat16 *v = static_cast<const __nv_bfloat16 *>(p.v) + k0 * p.ldv + (long long)(head / p.group) * p.dim;
+  for (int d = 0; d < p.dim; d += 8) {
+    float sum[8] = {};
+    for (int j = j0; j < j1; ++j) {
+      const uint4 w = *reinterpret_cast<const uint4 *>(v + j * p.ldv + d);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t bits = e & 1 ? u[e / 2] & 0xffff0000u : u[e / 2] << 16;
+        if ((bits & 0x7f800000u) == 0x7f800000u) sum[e] += __uint_as_float(bits);
+      }
     }
-    for (int d = 0; d < 8; ++d) from_f32(y + d0 + d, n > 0 ? acc[d] / l : 0.f);
+    for (int e = 0; e < 8; ++e)
+      if (sum[e] != 0.f) y[d + e] = __float2bfloat16_rn(__bfloat162float(y[d + e]) + sum[e]);
   }
 }
 
@@ -718,12 +709,12 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       if (!ok) break;
       const long long q_row = (long long)t.q0 + query;
       const int all_heads = t.kh * p.group + head;
-      bool plain = false;
+      bool mend = false;   // add the values that were left out of the product
       if (begin < n) {
         if (!(ok = warp_wait(bar_o + 8 * x, results & 1, abort_flag))) break;
         ++results;
         tc_fence_after();
-        plain = unclean[i & 3] == i + 1;
+        mend = unclean[i & 3] == i + 1;
       }
       if (!busy) {
         if (begin < n && lane == 0) mbar_arrive(bar_oe + 8 * x);
@@ -750,7 +741,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           const __nv_bfloat162 h = none ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
           w[k] = *reinterpret_cast<const uint32_t *>(&h);
         }
-        if (!mine || plain) continue;
+        if (!mine) continue;
         if (sectors) {   // a lane's row leaves in whole 32-byte sectors
 #pragma unroll
           for (int k = 0; k < 16; k += 8)
@@ -764,7 +755,8 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             if (d + 2 * k < p.dim) *reinterpret_cast<uint4 *>(y + d + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
         }
       }
-      if (plain && mine) plain_row(p, q_row, all_heads, t.k0, lim);
+      if (mend && mine)   // the tile's first query sees all keys before lim - query: adding an infinity or NaN of those once more changes nothing
+        add_nonfinite(p, q_row, all_heads, t.k0, max(0, lim - query), lim);
     }
     if (!ok) {
       *abort_flag = 1;
@@ -891,7 +883,8 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             // The product takes 16 keys at a time and stops after the last one that anybody here sees.  Values past that key belong
             // to others and may hold anything: zeros in their place, since the tensor cores multiply every value by every row's
             // weight and 0 * NaN is NaN.  Values on the diagonal are hidden
-            // from some rows only: if one is not finite, the rows are summed up the plain way at the end.
+            // from some rows only: one that is not finite becomes zero here, and the rows that see it add it at the end (any weight
+            // above 0 leaves an infinity or NaN what it is).
             uint8_t *v = gen + QS * Cfg::Q + vs * Cfg::TILE;
             constexpr int PIECES = 8 * Cfg::PANELS;   // 16-byte pieces of a key's values
             const int none = max(0, min(KEYS, lim_hi - base)), some = max(0, min(none, lim_lo - base));
@@ -905,7 +898,15 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               const uint4 w = *reinterpret_cast<const uint4 *>(v + (piece >> 3) * Cfg::PANEL + key * 128 + (piece & 7) * 16);
               for (uint32_t u : {w.x, w.y, w.z, w.w}) bad |= (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
             }
-            if (bad) unclean[i & 3] = i + 1;   // this warp is at most two tiles ahead: the mail has two places
+            if (__any_sync(0xffffffffu, bad)) {
+              unclean[i & 3] = i + 1;   // this warp is at most two tiles ahead: the mail has two places
+#pragma unroll 1
+              for (int k = some * PIECES * 4 + lane; k < none * PIECES * 4; k += 32) {   // words
+                const int key = k / (PIECES * 4), word = k % (PIECES * 4);
+                uint32_t *w = reinterpret_cast<uint32_t *>(v + (word >> 5) * Cfg::PANEL + key * 128 + (word & 31) * 4);
+                *w &= ((*w & 0x7f80u) == 0x7f80u ? 0xffff0000u : 0xffffffffu) & ((*w & 0x7f800000u) == 0x7f800000u ? 0xffffu : 0xffffffffu);
+              }
+            }
             fence_proxy_async();
             __syncwarp();
           }
@@ -1069,7 +1070,7 @@ int sofie_b200_prompt_attention_enqueue(sofie_b200_prompt_attention_plan *plan, 
                                         int64_t k_tokens) {
   if (!plan) return fail(SOFIE_B200_ERR_INVALID, "prompt_attention_enqueue: plan is NULL");
   const sofie_b200_prompt_attention_desc &d = plan->d;
-  if (batch < 0 || batch > 0x3fffffff || q_tokens < 0 || q_tokens > 0x3fffffff || k_tokens < 0 || k_tokens > 0x3fffffff)
+  if (batch < 0 || batch > 0x3fffffff || q_tokens < 0 || q_tokens > (1 << 27) || k_tokens < 0 || k_tokens > (1 << 27))   // a warp without rows waits for a tile's others: within the limit
     return fail(SOFIE_B200_ERR_INVALID, "prompt_attention_enqueue: bad extent (batch %lld, %lld and %lld tokens)", (long long)batch,
                 (long long)q_tokens, (long long)k_tokens);
   if (batch == 0 || q_tokens == 0) return 0;

@@ -131,10 +131,10 @@ def test_python_handles_refuse(b200_lib):
     for bad, text in ((z(5, 4, 64).transpose(1, 2), "one behind another"), (z(5, 8, 64)[:, ::2], "one behind another"), (z(5, 64), "is expected"),
                       (z(5, 12, 64)[:, 2:6], "CUDA")):
         with pytest.raises(ValueError, match=text):
-            ops._rows("x", bad)
+            ops._rows("x", bad, 0)
     for bad in (z(4, dt=torch.int32), z(3), z(3, 1, dt=torch.int32), z(6, dt=torch.int32)[::2], z(3, dt=torch.int32)):   # the last: not on a GPU
         with pytest.raises(ValueError):
-            ops._offsets("cu", bad, 2)
+            ops._offsets("cu", bad, 2, 0)
 
 
 HOSTILE = r'''

@@ -162,6 +162,56 @@ def test_append_leaves_out_bad_pages_and_positions(ctx):
     assert torch.equal(ck, keep)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_in_place(ctx, dtype, interleaved):
+    """q_out = q and k_out = k, column blocks of one tensor: the bits of the call with outputs of their own, the values untouched."""
+    from sofie_b200.ops import PagedKV
+    g = gen_of(61)
+    for heads, kvh, dim, rotary in ((6, 2, 64, 64), (3, 1, 40, 24), (2, 1, 9, 6)):
+        lens, n = [30, 7], 37
+        table, pages = ref.make_pages(lens, 16, g)
+        cos, sin = tables(40, rotary)
+        qkv = normal(g, (n, heads + 2 * kvh, dim), dtype)
+        before = qkv.clone()
+        caches = []
+        for inplace in (False, True):
+            ck, cv = (torch.zeros((pages, 16, kvh, dim), dtype=dtype, device=DEV) for _ in range(2))
+            q, k, v = qkv[:, :heads], qkv[:, heads:heads + kvh], qkv[:, heads + kvh:]
+            qo, ko = (q, k) if inplace else (torch.empty((n, heads, dim), dtype=dtype, device=DEV), torch.empty((n, kvh, dim), dtype=dtype, device=DEV))
+            ctx.kv_append(k, v, PagedKV(ck, cv, table, ints(lens)), ints([0, 30, 37]), cos=cos, sin=sin, interleaved=interleaved, q=q, q_out=qo, k_out=ko)
+            ctx.sync()
+            caches.append((ck, cv, qo.clone(), ko.clone()))
+            if not inplace:
+                assert torch.equal(qkv, before)
+        for a, b in zip(*caches):
+            assert torch.equal(a, b)
+        assert torch.equal(qkv[:, heads + kvh:], before[:, heads + kvh:])
+
+
+def test_append_many_sequences(ctx):
+    """More sequences than a warp looks at in one round or in two, many of them without a new token."""
+    from sofie_b200.ops import PagedKV
+    for batch in (33, 1025, 3000):
+        g = gen_of(batch)
+        new = torch.randint(0, 3, (batch,), generator=g, device=DEV).tolist()
+        past = torch.randint(0, 20, (batch,), generator=g, device=DEV).tolist()
+        total = [a + b for a, b in zip(past, new)]
+        table, pages = ref.make_pages(total, 4, g, width=6)
+        cu = offsets(new)
+        k, v = normal(g, (cu[-1] + 3, 1, 8), BF), normal(g, (cu[-1] + 3, 1, 8), BF)
+        ck, cv = (torch.zeros((pages, 4, 1, 8), dtype=BF, device=DEV) for _ in range(2))
+        wk, wv = ck.clone(), cv.clone()
+        rows = table.cpu()
+        for b in range(batch):
+            for i in range(new[b]):
+                pos = past[b] + i
+                wk[rows[b, pos // 4], pos % 4], wv[rows[b, pos // 4], pos % 4] = k[cu[b] + i], v[cu[b] + i]
+        ctx.kv_append(k, v, PagedKV(ck, cv, table, ints(total)), ints(cu))
+        ctx.sync()
+        assert torch.equal(ck, wk) and torch.equal(cv, wv)
+
+
 # ---- prompts --------------------------------------------------------------------------------------------------------
 PROMPT = [
     # heads, kv_heads, dim, causal, query lengths, key lengths (None: the same)
@@ -243,6 +293,45 @@ def test_prompt_hidden_keys_have_no_influence(ctx, dtype, heads, kvh, dim):
     late = v[90].double().sign() * math.inf
     assert (y[90:100].double() == late[0, 0]).all()
     assert torch.isnan(y[215:220, :, 3]).all() and torch.isfinite(y[215:220, :, :3]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("heads,kvh,dim", [(3, 1, 64), (1, 1, 8), (4, 2, 128), (1, 1, 104), (2, 1, 256)])
+def test_prompt_values_that_are_not_finite(ctx, dtype, heads, kvh, dim):
+    """Single infinite and NaN values all along a prompt: the queries from them on have them in that dimension, everything else is what
+    it is without them."""
+    from sofie_b200.ops import PromptAttentionPlan
+    lens = [9, 701]
+    q, k, v, cq, _ = prompt_case(heads, kvh, dim, lens, None, dtype, 13)
+    clean = v.clone()
+    for at, d, value in ((3, 0, math.inf), (9 + 10, 7, -math.inf), (9 + 300, 2, math.inf), (9 + 305, 2, -math.inf), (9 + 500, 5, math.inf), (9 + 601, dim - 2, math.nan),
+                         (9 + 700, 1, math.inf)):
+        v[at, :, d], clean[at, :, d] = value, 0.0
+    want, tol = ref.prompt(q, k, clean, cq, cq, True)
+    y = torch.zeros_like(q)
+    PromptAttentionPlan(ctx, heads, kvh, dim, dtype).enqueue(q, k, v, y, ints(cq))
+    ctx.sync()
+    for first, end, d, value in ((3, 9, 0, math.inf), (19, 710, 7, -math.inf), (309, 314, 2, math.inf), (314, 710, 2, math.nan), (509, 710, 5, math.inf),
+                                 (610, 710, dim - 2, math.nan), (709, 710, 1, math.inf)):
+        got = y[first:end, :, d].double()
+        assert (got.isnan() if math.isnan(value) else got == value).all(), (first, d)
+        want[first:end, :, d], y[first:end, :, d] = 0.0, 0.0
+    ref.close(y[:710], want[:710], tol[:710])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_prompt_many_sequences(ctx, dtype):
+    """More sequences than the blocks' table has places, most of them a few tokens, some of them none."""
+    from sofie_b200.ops import PromptAttentionPlan
+    g = gen_of(17)
+    lens = torch.randint(0, 9, (1000,), generator=g, device=DEV).tolist()
+    lens[500], lens[999] = 400, 130
+    q, k, v, cq, _ = prompt_case(4, 2, 64, lens, None, dtype, 17)
+    want, tol = ref.prompt(q, k, v, cq, cq, True)
+    y = torch.zeros_like(q)
+    PromptAttentionPlan(ctx, 4, 2, 64, dtype).enqueue(q, k, v, y, ints(cq))
+    ctx.sync()
+    ref.close(y[:cq[-1]], want[:cq[-1]], tol[:cq[-1]])
 
 
 def test_prompt_rows_far_from_the_maximum(ctx):
@@ -404,6 +493,23 @@ def test_decode_leaves_out_bad_pages(ctx):
         assert (y[0] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_decode_shared_pages(ctx, dtype):
+    """A common prefix: sequences that share pages, one page twice in a sequence, a table with a pitch of its own."""
+    from sofie_b200.ops import PagedAttentionPlan, PagedKV
+    g = gen_of(23)
+    ck, cv = normal(g, (12, 16, 2, 64), dtype), normal(g, (12, 16, 2, 64), dtype)
+    wide = torch.full((3, 9), 99, dtype=torch.int32, device=DEV)
+    table = wide[:, 2:7]
+    table.copy_(ints([[3, 4, 5, 6, 0], [3, 4, 5, 7, 0], [8, 8, 3, 8, 1]]))
+    lens = [61, 64, 80]
+    q = normal(g, (3, 8, 64), dtype)
+    y = torch.empty_like(q)
+    PagedAttentionPlan(ctx, 8, 2, 64, dtype).enqueue(q, PagedKV(ck, cv, table, ints(lens)), y)
+    ctx.sync()
+    ref.close(y, *ref.decode(q, ck, cv, table, lens))
+
+
 def test_far_pages(ctx):
     """Cache offsets past 2^31 elements: append there and read it back."""
     from sofie_b200.ops import PagedAttentionPlan, PagedKV
@@ -535,6 +641,53 @@ def test_two_streams_at_once(b200_lib):
         ref.close(y, want, tol)
         plan.close()
         c.close()
+
+
+def test_two_graphs_replayed_side_by_side(b200_lib):
+    """Two plans, each captured into a graph of its own, replayed on two streams at once."""
+    from sofie_b200.ops import Context, PagedAttentionPlan, PagedKV, PromptAttentionPlan
+    runs = []
+    for i in range(2):
+        s = torch.cuda.Stream(device=DEV)
+        c = Context(0, stream=s)
+        lens = [5000 - 700 * i, 3, 1200]
+        q, ck, cv, table = decode_case(8, 2, 128, 16, lens, False, BF, 70 + i)
+        qp, kp, vp, cq, _ = prompt_case(8, 2, 128, [300, 40 + i], None, BF, 80 + i, spare=0)
+        kv, y, yp, cu = PagedKV(ck, cv, table, ints(lens)), torch.empty_like(q), torch.empty_like(qp), ints(cq)
+        plan, prompt = PagedAttentionPlan(c, 8, 2, 128, BF), PromptAttentionPlan(c, 8, 2, 128, BF)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            for _ in range(3):
+                plan.enqueue(q, kv, y)
+                prompt.enqueue(qp, kp, vp, yp, cu)
+        runs.append((s, c, graph, plan, prompt, y, yp, ref.decode(q, ck, cv, table, lens), ref.prompt(qp, kp, vp, cq, cq, True), (q, kv, qp, kp, vp, cu)))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, c, graph, *_r in runs:
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for s, c, graph, plan, prompt, y, yp, d, pr, _keep in runs:
+        c.sync()
+        ref.close(y, *d)
+        ref.close(yp, *pr)
+    for r in runs:
+        r[2].reset()
+        r[3].close()
+        r[4].close()
+        r[1].close()
+
+
+def test_prompt_extents_that_are_refused(ctx):
+    from sofie_b200.ops import PromptAttentionPlan
+    q = torch.empty((8, 1, 8), dtype=BF, device=DEV)
+    cu = ints([0, 8])
+    plan = PromptAttentionPlan(ctx, 1, 1, 8, BF)
+    for batch, n, m in ((-1, 8, 8), (1, -1, 8), (1, 8, -1), (1, (1 << 27) + 1, 8), (1, 8, (1 << 27) + 1), (1 << 30, 8, 8)):
+        p = q.data_ptr()
+        assert L.load().sofie_b200_prompt_attention_enqueue(plan._plan((0, 0, 0, 0)), p, p, p, p, cu.data_ptr(), cu.data_ptr(), batch, n, m) == L.ERR_INVALID
+    ctx.sync()
 
 
 def test_refusals_with_a_context(ctx):
