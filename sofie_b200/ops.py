@@ -189,24 +189,27 @@ class Context:
         packed, for PromptAttentionPlan.  cos, sin: fp32 [positions, rotary_dim / 2], absent = no rotation.  cu_seqlens: int32
         [batch + 1], the packed rows of each sequence; absent = one token per sequence.  Token rows may be column blocks of a
         wider tensor.  q_out may be q, k_out may be k."""
-        tokens, kv_heads, dim, ldk, pk = _rows("k", k)
+        dev = self.device
+        tokens, kv_heads, dim, ldk, pk = _rows("k", k, dev)
         dtype = k.dtype
+        if kv._device != dev:
+            _wrong_device("kv_append: the cache", kv.k, dev)
         if kv_heads != kv.kv_heads or dim != kv.head_dim or dtype is not kv.dtype:
             raise ValueError(f"kv_append: keys of {kv_heads} heads of {dim} {dtype}, cache of {kv.kv_heads} of {kv.head_dim} {kv.dtype}")
-        n, h, e, ldv, pv = _rows("v", v)
+        n, h, e, ldv, pv = _rows("v", v, dev)
         if n != tokens or h != kv_heads or e != dim or v.dtype is not dtype:
             raise ValueError(f"kv_append: values {tuple(v.shape)} {v.dtype} beside keys {tuple(k.shape)} {dtype}")
         ldko = heads = ldq = ldqo = rotary = positions = 0
         pko = pq = pqo = pcos = psin = pcu = None
         if k_out is not None:
-            n, h, e, ldko, pko = _rows("k_out", k_out)
+            n, h, e, ldko, pko = _rows("k_out", k_out, dev)
             if n != tokens or h != kv_heads or e != dim or k_out.dtype is not dtype:
                 raise ValueError(f"kv_append: k_out {tuple(k_out.shape)} {k_out.dtype} beside keys {tuple(k.shape)} {dtype}")
         if q is not None:
             if q_out is None:
                 raise ValueError("kv_append: q needs q_out")
-            n, heads, e, ldq, pq = _rows("q", q)
-            m, h, f, ldqo, pqo = _rows("q_out", q_out)
+            n, heads, e, ldq, pq = _rows("q", q, dev)
+            m, h, f, ldqo, pqo = _rows("q_out", q_out, dev)
             if n != tokens or e != dim or q.dtype is not dtype:
                 raise ValueError("kv_append: q and k differ in tokens, head size or type")
             if m != tokens or h != heads or f != dim or q_out.dtype is not dtype:
@@ -221,9 +224,11 @@ class Context:
             positions, rotary = cos.shape
             rotary *= 2
             if rotary:
-                pcos, psin = _ptr(cos), _ptr(sin)
+                if cos.get_device() != dev or sin.get_device() != dev:
+                    _wrong_device("kv_append: cos and sin", cos if cos.get_device() != dev else sin, dev)
+                pcos, psin = cos.data_ptr(), sin.data_ptr()
         if cu_seqlens is not None:
-            pcu = _offsets("cu_seqlens", cu_seqlens, kv.batch)
+            pcu = _offsets("cu_seqlens", cu_seqlens, kv.batch, dev)
         d = L.KvAppendDesc(tokens, heads, kv_heads, dim, rotary, 1 if interleaved else 0, kv._dtype_code, positions, ldq, ldk, ldv, ldqo, ldko)
         status = self._lib.sofie_b200_kv_append_enqueue(self._h, C.byref(d), kv._ref, pcu, pq, pk, pv, pcos, psin, pqo, pko)
         if status:
@@ -250,9 +255,9 @@ class Context:
                 "convert_enqueue")
 
 
-def _rows(name, t):
-    """(tokens, heads, head size, token pitch, address) of a [tokens, heads, head_dim] tensor on the GPU whose rows may be column
-    blocks of wider ones."""
+def _rows(name, t, device):
+    """(tokens, heads, head size, token pitch, address) of a [tokens, heads, head_dim] tensor on GPU `device` whose rows may be
+    column blocks of wider ones."""
     shape = t.shape
     if len(shape) != 3:
         raise ValueError(f"{name}: [tokens, heads, head_dim] is expected, not {tuple(shape)}")
@@ -260,16 +265,24 @@ def _rows(name, t):
     sn, sh, sd = t.stride()
     if (sd != 1 and d > 1) or (sh != d and h > 1):
         raise ValueError(f"{name}: the heads of a token must lie one behind another (strides {t.stride()})")
-    if not t.is_cuda:
-        raise ValueError("sofie_b200 operators take CUDA tensors; host data goes through run_host()")
+    if t.get_device() != device:
+        _wrong_device(name, t, device)
     return n, h, d, sn if n > 1 else h * d, t.data_ptr()
 
 
-def _offsets(name, t, batch):
-    """Address of an int32 tensor of batch + 1 row offsets on the GPU."""
+def _wrong_device(name, t, device):
+    if not t.is_cuda:
+        raise ValueError("sofie_b200 operators take CUDA tensors; host data goes through run_host()")
+    raise ValueError(f"{name}: on {t.device}, the context's device is cuda:{device}")
+
+
+def _offsets(name, t, batch, device):
+    """Address of an int32 tensor of batch + 1 row offsets on GPU `device`."""
     if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != batch + 1 or not t.is_contiguous():
         raise ValueError(f"{name}: a contiguous int32 tensor of batch + 1 = {batch + 1} row offsets is expected")
-    return _ptr(t)
+    if t.get_device() != device:
+        _wrong_device(name, t, device)
+    return t.data_ptr()
 
 
 class PagedKV:
@@ -293,7 +306,7 @@ class PagedKV:
             raise ValueError("PagedKV: all tensors live on one device")
         self.k, self.v, self.block_table, self.seq_lens = k, v, block_table, seq_lens
         self.kv_heads, self.head_dim, self.dtype, self.batch = kv_heads, dim, k.dtype, seq_lens.shape[0]
-        self._dtype_code = dtype_code(k.dtype)
+        self._dtype_code, self._device = dtype_code(k.dtype), k.get_device()
         width = block_table.shape[1]
         # the stride of an axis of one element says nothing: the dense one stands for it
         hs = k.stride(2) if kv_heads > 1 else dim
@@ -330,11 +343,11 @@ class PromptAttentionPlan:
     def enqueue(self, q, k, v, y, cu_seqlens, cu_seqlens_k=None) -> None:
         """q, y: [tokens, heads, head_dim]; k, v: [key tokens, kv_heads, head_dim], rows packed sequence behind sequence;
         cu_seqlens (and cu_seqlens_k, where keys have other lengths than queries): int32 [batch + 1] row offsets."""
-        dtype = self._dtype
-        n, h, d, ldq, pq = _rows("q", q)
-        nk, hk, dk, ldk, pk = _rows("k", k)
-        nv, hv, dv, ldv, pv = _rows("v", v)
-        ny, hy, dy, ldy, py = _rows("y", y)
+        dtype, dev = self._dtype, self.ctx.device
+        n, h, d, ldq, pq = _rows("q", q, dev)
+        nk, hk, dk, ldk, pk = _rows("k", k, dev)
+        nv, hv, dv, ldv, pv = _rows("v", v, dev)
+        ny, hy, dy, ldy, py = _rows("y", y, dev)
         if (h, hk, d) != self._shape or dk != d or nv != nk or hv != hk or dv != d or ny != n or hy != h or dy != d:
             raise ValueError(f"prompt attention: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, y {tuple(y.shape)} do not match the plan")
         if q.dtype is not dtype or k.dtype is not dtype or v.dtype is not dtype or y.dtype is not dtype:
@@ -342,8 +355,8 @@ class PromptAttentionPlan:
         batch = cu_seqlens.numel() - 1
         if batch < 0:
             raise ValueError("cu_seqlens: batch + 1 row offsets are expected")
-        pcu = _offsets("cu_seqlens", cu_seqlens, batch)
-        pck = _offsets("cu_seqlens_k", cu_seqlens_k, batch) if cu_seqlens_k is not None else None
+        pcu = _offsets("cu_seqlens", cu_seqlens, batch, dev)
+        pck = _offsets("cu_seqlens_k", cu_seqlens_k, batch, dev) if cu_seqlens_k is not None else None
         status = self._lib.sofie_b200_prompt_attention_enqueue(self._plan((ldq, ldk, ldv, ldy)), pq, pk, pv, py, pcu, pck, batch, n, nk)
         if status:
             L.check(status, "prompt_attention_enqueue")
@@ -394,12 +407,14 @@ class PagedAttentionPlan:
 
     def enqueue(self, q, kv, y) -> None:
         """q, y: [batch, heads, head_dim]; kv: the PagedKV with the cache and its batch of sequences."""
-        dtype = self._dtype
-        n, h, d, ldq, pq = _rows("q", q)
-        ny, hy, dy, ldy, py = _rows("y", y)
+        dtype, dev = self._dtype, self.ctx.device
+        n, h, d, ldq, pq = _rows("q", q, dev)
+        ny, hy, dy, ldy, py = _rows("y", y, dev)
         if (h, kv.kv_heads, d) != self._shape or kv.head_dim != d or n != kv.batch or q.dtype is not dtype or kv.dtype is not dtype:
             raise ValueError(f"paged attention: q {tuple(q.shape)} {q.dtype} over {kv.batch} sequences of {kv.kv_heads} heads of {kv.head_dim} "
                              f"{kv.dtype} does not match the plan")
+        if kv._device != dev:
+            _wrong_device("paged attention: the cache", kv.k, dev)
         if ny != n or hy != h or dy != d or y.dtype is not dtype:
             raise ValueError(f"paged attention: y {tuple(y.shape)} {y.dtype} beside q {tuple(q.shape)} {dtype}")
         status = self._lib.sofie_b200_paged_attention_enqueue(self._plan((ldq, ldy)), pq, kv._ref, py, self._workspace_ptr)
