@@ -120,22 +120,24 @@ __device__ __forceinline__ int seen(const PromptParams &p, const PromptTile &t, 
 }
 
 // ---- fp32 on the CUDA cores --------------------------------------------------------------------------------------------------------
-// A block computes 32 rows; each of its teams of four warps takes every TEAMS-th tile of 64 keys, and the teams' sums are joined at the end.
-// (Few blocks are long chains of tiles on few warps otherwise: 770 queries of 8 heads over 1770 keys take 80 us with one team, 71 us with
-// two; prompts of 2048 tokens 31 TFLOP/s, 0.42 of the FMA pipes, with either.  Above head size 128 a second team's tiles do not fit.)
+// A block computes 32 rows; each of its teams of four warps takes every TEAMS-th tile of 64 keys, and the teams' sums are joined at the end
+// (where blocks are few, those of a cluster of them too, through distributed shared memory).
+// (Few blocks are long chains of tiles on few warps otherwise: 770 queries of 8 heads over 1770 keys take 80 us with one team, 71 with
+// two, 61 with two blocks of two; prompts of 2048 tokens 31 TFLOP/s, 0.42 of the FMA pipes, with any.  Above head size 128 a second
+// team's tiles do not fit.)
 // A thread has 4 rows x 4 keys of the scores and 4 rows x DP / 16 dimensions of the result, so that a 16-byte read from shared memory
 // feeds 16 FMAs and the FMA pipes are what bounds it.  The next keys arrive while this tile's values are weighed, the next values while
 // the next scores are computed (cp.async, one place each).
 constexpr int PF_ROWS = 32, PF_KEYS = 64, PF_TEAM = 128;
 template <int DP>
 struct FmaCfg {
-  static constexpr int TEAMS = DP <= 128 ? 2 : 1, THREADS = TEAMS * PF_TEAM;
+  static constexpr int TEAMS = DP <= 128 ? 2 : 1, THREADS = TEAMS * PF_TEAM, BLOCKS = DP == 64 ? 2 : 1;   // BLOCKS: that fit an SM
   static constexpr int Q = PF_ROWS * DP * 4, TILE = PF_KEYS * DP * 4, P = PF_KEYS * PF_ROWS * 4;
   static constexpr int SMEM = Q + TEAMS * (2 * TILE + P) + 4 * (RUNS + 1);
 };
 
 template <int DP>
-__global__ void __launch_bounds__(FmaCfg<DP>::THREADS) prompt_fma_kernel(const __grid_constant__ PromptParams p, int parts) {
+__global__ void __launch_bounds__(FmaCfg<DP>::THREADS) prompt_fma_kernel(const __grid_constant__ PromptParams p, int parts, int share) {
   using Cfg = FmaCfg<DP>;
   constexpr int CH = DP / 4, PIECES = DP / 64;   // 16-byte pieces of a row; of the result per thread and row
   extern __shared__ __align__(128) uint8_t smem[];
@@ -144,7 +146,8 @@ __global__ void __launch_bounds__(FmaCfg<DP>::THREADS) prompt_fma_kernel(const _
   int *table = reinterpret_cast<int *>(smem + Cfg::Q + Cfg::TEAMS * (2 * Cfg::TILE + Cfg::P));
   auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(PF_TEAM) : "memory"); };   // the team
   count_tiles(p, table);
-  const int work = blockIdx.x / parts, part = blockIdx.x % parts, kh = work % p.kv_heads;   // a group of more than 32 heads is several parts
+  const int block = blockIdx.x / share, rank = blockIdx.x % share;
+  const int work = block / parts, part = block % parts, kh = work % p.kv_heads;   // a group of more than 32 heads is several parts
   const PromptTile t = find_tile(p, table, work / p.kv_heads);
   if (t.queries == 0) return;
   const int head0 = part * PF_ROWS, heads = min(PF_ROWS, p.group - head0);   // heads of the group in this block
@@ -163,7 +166,7 @@ __global__ void __launch_bounds__(FmaCfg<DP>::THREADS) prompt_fma_kernel(const _
       cp_async_16(dst + (r * CH + (swizzle ? c ^ (r & 7) : c)) * 16, src + (there ? (base + r) * pitch + c * 4 : 0), there);
     }
   };
-  const int begin = n - 1 - team;   // this team's tiles: begin, begin - TEAMS, ...
+  const int stride = Cfg::TEAMS * share, begin = n - 1 - (rank * Cfg::TEAMS + team);   // this team's tiles: begin, begin - stride, ...
   for (int i = threadIdx.x; i < PF_ROWS * CH; i += Cfg::THREADS) {
     const int r = i / CH, c = i % CH, query = r / heads, h = r - query * heads;
     const bool there = query < t.queries && c * 4 < p.dim;
@@ -191,7 +194,7 @@ __global__ void __launch_bounds__(FmaCfg<DP>::THREADS) prompt_fma_kernel(const _
     for (int j = 0; j < PIECES; ++j) acc[r][j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 
-  for (int it = begin; it >= 0; it -= Cfg::TEAMS) {
+  for (int it = begin; it >= 0; it -= stride) {
     const int base = it * PF_KEYS;
     const bool masked = base + PF_KEYS > lim_lo;
     cp_async_wait<1>();   // the keys
@@ -210,7 +213,7 @@ __global__ void __launch_bounds__(FmaCfg<DP>::THREADS) prompt_fma_kernel(const _
         for (int j = 0; j < 4; ++j) s[r][j] = fmaf(a[r].x, b[j].x, fmaf(a[r].y, b[j].y, fmaf(a[r].z, b[j].z, fmaf(a[r].w, b[j].w, s[r][j]))));
     }
     meet();   // the keys are read
-    if (it >= Cfg::TEAMS) load_tile(a_k, k, p.ldk, base - Cfg::TEAMS * PF_KEYS, true);
+    if (it >= stride) load_tile(a_k, k, p.ldk, base - stride * PF_KEYS, true);
     cp_async_commit();
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -281,35 +284,62 @@ __global__ void __launch_bounds__(FmaCfg<DP>::THREADS) prompt_fma_kernel(const _
       }
     }
     meet();   // values and weights are read
-    if (it >= Cfg::TEAMS) load_tile(a_v, v, p.ldv, base - Cfg::TEAMS * PF_KEYS, false);
+    if (it >= stride) load_tile(a_v, v, p.ldv, base - stride * PF_KEYS, false);
     cp_async_commit();
   }
   cp_async_wait<0>();
-  if constexpr (Cfg::TEAMS == 2) {   // the second team's sums onto the first one's, thread by thread
-    float4 *sum = reinterpret_cast<float4 *>(smem + Cfg::Q + (2 * Cfg::TILE + Cfg::P));   // the second team's keys, which are read
-    if (team == 1) {
-      meet();
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        sum[(r * (PIECES + 1)) * PF_TEAM + tid] = make_float4(m[r], l[r], 0.f, 0.f);
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j) sum[(r * (PIECES + 1) + 1 + j) * PF_TEAM + tid] = acc[r][j];
-      }
-    }
-    __syncthreads();
-    if (team == 1) return;
+  // Sums meet thread by thread: a thread's rows and dimensions are the same in every team and block.  They lie where the last team's
+  // keys were, which are read.
+  constexpr int PLACE = Cfg::Q + (Cfg::TEAMS - 1) * (2 * Cfg::TILE + Cfg::P);
+  float4 *sum = reinterpret_cast<float4 *>(smem + PLACE) + tid;
+  auto leave = [&]() {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const float4 ml = sum[(r * (PIECES + 1)) * PF_TEAM + tid];
+      sum[r * (PIECES + 1) * PF_TEAM] = make_float4(m[r], l[r], 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) sum[(r * (PIECES + 1) + 1 + j) * PF_TEAM] = acc[r][j];
+    }
+  };
+  auto join = [&](auto fetch) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float4 ml = fetch(r * (PIECES + 1) * PF_TEAM);
       const float top = fmaxf(m[r], ml.x), off = top == -INFINITY ? 0.f : top, f = ex2(m[r] - off), g2 = ex2(ml.x - off);
       m[r] = top;
       l[r] = l[r] * f + ml.y * g2;
 #pragma unroll
       for (int j = 0; j < PIECES; ++j) {
-        const float4 x = sum[(r * (PIECES + 1) + 1 + j) * PF_TEAM + tid];
+        const float4 x = fetch((r * (PIECES + 1) + 1 + j) * PF_TEAM);
         acc[r][j] = make_float4(acc[r][j].x * f + x.x * g2, acc[r][j].y * f + x.y * g2, acc[r][j].z * f + x.z * g2, acc[r][j].w * f + x.w * g2);
       }
     }
+  };
+  if constexpr (Cfg::TEAMS == 2) {
+    if (team == 1) {
+      meet();
+      leave();
+    }
+    __syncthreads();
+    if (team == 1) return;
+    join([&](int i) { return sum[i]; });
+  }
+  if (share > 1) {   // the cluster's blocks: the first one takes the others' sums, in order
+    meet();          // with one team: its keys are read; with two: so are the second one's sums, by their own threads
+    if (rank > 0) leave();
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank == 0) {
+      for (int other = 1; other < share; ++other) {
+        uint32_t at;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(sum)), "r"(other));
+        join([&](int i) {
+          float4 x;
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at + i * 16) : "memory");
+          return x;
+        });
+      }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // and they stay until it has
+    if (rank > 0) return;
   }
 
 #pragma unroll
@@ -1011,8 +1041,24 @@ static int launch_fma(sofie_b200_ctx *ctx, PromptParams p) {
   if (grid > 0x7fffffffLL) return fail(SOFIE_B200_ERR_TOO_LARGE, "prompt_attention_enqueue: %lld queries of %d heads", p.q_rows, p.heads);
   if (!p.k_rows) p.k = p.v = p.q;   // nothing is read, but the address a copy of no bytes is given should exist
   SB_CUDA(cudaFuncSetAttribute(prompt_fma_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, FmaCfg<DP>::SMEM));   // per device
-  prompt_fma_kernel<DP><<<(unsigned)grid, FmaCfg<DP>::THREADS, FmaCfg<DP>::SMEM, ctx->stream>>>(p, parts);
-  SB_CUDA(cudaGetLastError());
+  // Few blocks over many keys: clusters of 2, 4 or 8 share the keys of a tile of rows, as long as the blocks fill the GPU at most one and a half
+  // times and every team gets a tile of keys.  One block against two: 770 queries of 8 heads over 1770 keys 70 us, 61; 300 queries 21, 19;
+  // 20 queries over 2020 keys 99, 56 (four 33, eight 22); but 100 queries 12.9, 13.1; 300 of 16 heads of 128 33, 45; 2048 of 16 heads 290, 316.
+  int share = 1;
+  while (share < 8 && grid * share * 2 <= (long long)ctx->sm_count * FmaCfg<DP>::BLOCKS * 3 / 2 && p.k_rows / p.batch >= share * 2 * FmaCfg<DP>::TEAMS * PF_KEYS)
+    share *= 2;
+  cudaLaunchAttribute together{};
+  together.id = cudaLaunchAttributeClusterDimension;
+  together.val.clusterDim.x = share;
+  together.val.clusterDim.y = together.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(grid * share));
+  cfg.blockDim = dim3(FmaCfg<DP>::THREADS);
+  cfg.dynamicSmemBytes = FmaCfg<DP>::SMEM;
+  cfg.stream = ctx->stream;
+  cfg.attrs = &together;
+  cfg.numAttrs = share > 1;
+  SB_CUDA(cudaLaunchKernelEx(&cfg, prompt_fma_kernel<DP>, p, parts, share));
   ctx->launches++;
   return 0;
 }

@@ -232,6 +232,9 @@ PROMPT = [
     (2, 2, 104, True, [129], [513]),
     (12, 1, 128, True, [1] * 40, [5] * 40),
     (8, 2, 128, True, [1200], [2048]),
+    (2, 1, 64, True, [21], [2100]),
+    (3, 1, 128, False, [40, 9], [900, 1200]),
+    (2, 2, 256, True, [33], [700]),
 ]
 
 
