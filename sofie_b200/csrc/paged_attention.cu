@@ -20,7 +20,8 @@ using namespace ptx;
 
 constexpr int PA_UNIT = 16;       // keys
 constexpr int PA_ROWS = 16;       // query heads of an item at most: the rows of one mma tile
-constexpr int PA_LEAST = 3;       // slots that are worth a worker of their own
+constexpr int PA_LEAST = 3;       // slots that are worth a worker of their own.  2, 3, 4, 6, 9: few short sequences in fp32 17, 19, 21, 24, 29 us;
+                                  // one of 3000 tokens in bf16 20.6, 17.2, 19.1, 21.1, 23.2 us
 constexpr float PA_MARGIN = 16.f; // the reference maximum moves when a score is 2^16 above it: fp32 keeps its relative precision up there
 
 struct PagedAttnParams {
@@ -202,6 +203,9 @@ struct Bf16Cfg {
 // bf16.  Scores and weighted values on mma.m16n8k16 with the 16 rows = query heads of the group (rows past the group cost nothing that HBM
 // would not wait for).  The weights of the second product are split into two bf16 terms, high + low (error 2^-16 instead of 2^-8):
 // the tensor cores have the time.
+// Bound by HBM; at head size 128 the rings of two blocks are 192 KB an SM, two thirds of it on the way.  160 sequences, 1.22 GB of cache:
+// 209 to 230 us, 5.3 to 5.8 TB/s (DRAM 75 % busy, issue slots 42 %, tensor pipe 28 %); one of 65,543 tokens, 268 MB: 61 us with the launch of
+// both kernels, 4.4 TB/s.  A fixed split of every sequence into equal parts, one block each: 66 and 236 us.
 template <int DP>
 __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ PagedAttnParams p) {
   using Cfg = Bf16Cfg<DP>;
@@ -361,7 +365,8 @@ struct F32Cfg {
 
 // fp32, on the CUDA cores.  Scores: a lane has one key and half of its dimensions, the queries are read from shared memory by all lanes
 // at once; weights go through shared memory; weighted values: a lane has 4 dimensions (or, at head size 64, every other key of them).
-// R: query heads of an item at most.
+// R: query heads of an item at most.  Six sequences of up to 400 tokens, 2 key heads of 64: 18 us, the way of one launch after another
+// (the lengths, the table, a share of three units, the join), 0.38 MB.
 template <int DP, int R>
 __global__ void __launch_bounds__(F32Cfg<DP, R>::THREADS) paged_fma_kernel(const __grid_constant__ PagedAttnParams p) {
   using Cfg = F32Cfg<DP, R>;

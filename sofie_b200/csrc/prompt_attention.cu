@@ -518,6 +518,10 @@ __device__ __noinline__ void add_nonfinite(const PromptParams &p, long long q_ro
 // The reference maximum of a row moves only when a tile's maximum is 2^16 above it (fp32 and bf16 keep their relative precision up
 // there, and numerator and denominator use the same); then O is rescaled in tensor memory, which is rare.
 // Only tiles that the sequence's end or the diagonal cross pay for masks.  Every wait has a limit.
+// Measured: a causal prompt of 8192 tokens, 32 heads over 8 of 128, 494 to 505 us in bursts = 1.09 to 1.11 PFLOP/s (572 us under the power limit),
+// tensor pipe 51 % (60 % with its operand traffic), exponentials 51 %: the two rows' chains of maximum, exponential and hand-over
+// fill the gaps of one another only in part.  24 packed prompts of 5 to 2500 tokens 133 us; 512 sequences of 24 to 128, head size 64, full,
+// 131 MB: 60 us (a tile is two turns, so beginning and ending it is what counts).
 template <int DP>
 __global__ void __launch_bounds__(UmmaSize<DP>::THREADS, UmmaSize<DP>::BLOCKS)
 prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
