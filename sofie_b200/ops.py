@@ -265,6 +265,8 @@ def _rows(name, t, device):
     sn, sh, sd = t.stride()
     if (sd != 1 and d > 1) or (sh != d and h > 1):
         raise ValueError(f"{name}: the heads of a token must lie one behind another (strides {t.stride()})")
+    if n > 1 and sn < h * d:   # also a row expanded over all tokens: its stride, 0, is what the C side takes for "dense"
+        raise ValueError(f"{name}: rows lie over one another (strides {t.stride()}); an expanded tensor needs contiguous()")
     if t.get_device() != device:
         _wrong_device(name, t, device)
     return n, h, d, sn if n > 1 else h * d, t.data_ptr()
@@ -302,6 +304,10 @@ class PagedKV:
                 raise ValueError(f"PagedKV: {name} is an int32 tensor of rank {rank}, contiguous along its last axis")
         if block_table.shape[0] != seq_lens.shape[0]:
             raise ValueError("PagedKV: one row of the block table per sequence")
+        if block_table.shape[0] > 1 and block_table.stride(0) < block_table.shape[1]:   # 0, as expand leaves it, is "dense" to the C side
+            raise ValueError(f"PagedKV: rows of block_table lie over one another (strides {block_table.stride()}); an expanded table needs contiguous()")
+        if any(n > 1 and s == 0 for n, s in zip(k.shape[:3], k.stride())):
+            raise ValueError(f"PagedKV: elements of k and v lie over one another (strides {k.stride()})")
         if len({t.device for t in (k, v, block_table, seq_lens)}) != 1:
             raise ValueError("PagedKV: all tensors live on one device")
         self.k, self.v, self.block_table, self.seq_lens = k, v, block_table, seq_lens

@@ -137,6 +137,33 @@ def test_python_handles_refuse(b200_lib):
             ops._offsets("cu", bad, 2, 0)
 
 
+def test_rows_that_lie_over_one_another_are_refused(b200_lib):
+    """A row stride of 0 (one row expanded over a batch) or below a row's extent is no pitch: 0 means "dense" to the C entry points, which
+    would then read and write behind the tensor."""
+    from sofie_b200 import ops
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(s, dtype=dt)
+    for bad in (z(1, 4, 64).expand(5, 4, 64), z(1, 1, 64).expand(2, 1, 64), z(1, 4, 1).expand(3, 4, 1), z(1024).as_strided((5, 4, 64), (128, 64, 1)),
+                z(64).as_strided((2, 1, 64), (0, 64, 1))):
+        with pytest.raises(ValueError, match="over one another"):
+            ops._rows("x", bad, 0)
+    for fine in (z(1, 4, 64).expand(1, 4, 64), z(5, 4, 64)[:1], z(0, 4, 64)):      # a stride that is never taken says nothing
+        with pytest.raises(ValueError, match="CUDA"):
+            ops._rows("x", fine, 0)
+    lens, table, k = z(5, dt=torch.int32), z(5, 3, dt=torch.int32), z(4, 16, 2, 64)
+    for bad in (z(1, 3, dt=torch.int32).expand(5, 3), z(1, 1, dt=torch.int32).expand(5, 1), z(64, dt=torch.int32).as_strided((5, 3), (2, 1))):
+        with pytest.raises(ValueError, match="block_table.*over one another"):
+            ops.PagedKV(k, k, bad, lens)
+    for bad in (z(64).expand(4, 16, 2, 64), z(1, 16, 2, 64).expand(4, 16, 2, 64), z(4, 1, 2, 64).expand(4, 16, 2, 64), z(4, 16, 1, 64).expand(4, 16, 2, 64)):
+        with pytest.raises(ValueError, match="over one another"):
+            ops.PagedKV(bad, bad, table, lens)
+    for fine in (z(1, 3, dt=torch.int32).expand(1, 3), z(5, 9, dt=torch.int32)[:1, 2:5]):
+        with pytest.raises(ValueError, match="CUDA"):
+            ops.PagedKV(k, k, fine, lens[:1])
+    one = z(1, 1, 1, 64).expand(1, 1, 1, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.PagedKV(one, one, table, lens)
+
+
 HOSTILE = r'''
 #include "paged.cuh"
 #include <climits>
