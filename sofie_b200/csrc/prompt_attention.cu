@@ -665,6 +665,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         const bool masked = base + KEYS > lim_lo, first = it == begin;
         if (!busy) {
           if (Cfg::EARLY && lane == 0) mbar_arrive(bar_se + 8 * x);
+          __syncwarp();   // what follows (hand_over) takes all lanes
           // in step with the others: two turns ahead, its word would stand for one that is still at work
           if (Cfg::EARLY && !first && !(ok = warp_wait(bar_pv + 8 * x, (turns - 1) & 1, abort_flag))) break;
         } else {
@@ -677,6 +678,7 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_se + 8 * x);
+            __syncwarp();
             if (!first) {   // the previous product has left P and O
               if (!(ok = warp_wait(bar_pv + 8 * x, (turns - 1) & 1, abort_flag))) break;
               tc_fence_after();
@@ -775,19 +777,21 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
           const __nv_bfloat162 h = none ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(__uint_as_float(o[2 * k]) * inv, __uint_as_float(o[2 * k + 1]) * inv);
           w[k] = *reinterpret_cast<const uint32_t *>(&h);
         }
-        if (!mine) continue;
-        if (sectors) {   // a lane's row leaves in whole 32-byte sectors
+        if (mine) {
+          if (sectors) {   // a lane's row leaves in whole 32-byte sectors
 #pragma unroll
-          for (int k = 0; k < 16; k += 8)
-            if (d + 2 * k < p.dim)
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(y + d + 2 * k), "r"(w[k]), "r"(w[k + 1]), "r"(w[k + 2]), "r"(w[k + 3]),
-                           "r"(w[k + 4]), "r"(w[k + 5]), "r"(w[k + 6]), "r"(w[k + 7])
-                           : "memory");
-        } else {
+            for (int k = 0; k < 16; k += 8)
+              if (d + 2 * k < p.dim)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(y + d + 2 * k), "r"(w[k]), "r"(w[k + 1]), "r"(w[k + 2]), "r"(w[k + 3]),
+                             "r"(w[k + 4]), "r"(w[k + 5]), "r"(w[k + 6]), "r"(w[k + 7])
+                             : "memory");
+          } else {
 #pragma unroll
-          for (int k = 0; k < 16; k += 4)
-            if (d + 2 * k < p.dim) *reinterpret_cast<uint4 *>(y + d + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+            for (int k = 0; k < 16; k += 4)
+              if (d + 2 * k < p.dim) *reinterpret_cast<uint4 *>(y + d + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+          }
         }
+        __syncwarp();   // a warp that holds some rows only comes together again: the next load from tensor memory takes all its lanes
       }
       if (mend && mine)   // the tile's first query sees all keys before lim - query: adding an infinity or NaN of those once more changes nothing
         add_nonfinite(p, q_row, all_heads, t.k0, max(0, lim - query), lim);

@@ -337,6 +337,23 @@ def test_prompt_many_sequences(ctx, dtype):
     ref.close(y[:cq[-1]], want[:cq[-1]], tol[:cq[-1]])
 
 
+@pytest.mark.parametrize("heads,kvh,dim", [(3, 1, 64), (5, 1, 40), (7, 1, 80), (3, 1, 128), (6, 2, 72), (5, 1, 192), (3, 3, 256)])
+@pytest.mark.parametrize("gap", [0, 8])
+def test_prompt_warps_that_hold_some_rows_only(ctx, heads, kvh, dim, gap):
+    """Tiles that end inside a warp (groups that do not divide 32, sequences of every length up to a few), with rows of the result
+    that are stored in 32-byte pieces and in 16-byte ones; what lies between the rows stays."""
+    from sofie_b200.ops import PromptAttentionPlan
+    lens = [1, 2, 3, 5, 7, 11, 13, 31, 33, 43, 64, 85, 129]
+    q, k, v, cq, _ = prompt_case(heads, kvh, dim, lens, None, BF, dim + gap, spare=0)
+    want, tol = ref.prompt(q, k, v, cq, cq, True)
+    room = torch.full((cq[-1], heads * dim + gap), 3.0, dtype=BF, device=DEV)
+    y = room[:, :heads * dim].view(cq[-1], heads, dim)
+    PromptAttentionPlan(ctx, heads, kvh, dim, BF).enqueue(q, k, v, y, ints(cq))
+    ctx.sync()
+    ref.close(y, want, tol)
+    assert (room[:, heads * dim:] == 3.0).all()
+
+
 def test_prompt_rows_far_from_the_maximum(ctx):
     """Scores that grow along the keys by more than fp32's exponents hold: the running maximum has to follow."""
     from sofie_b200.ops import PromptAttentionPlan
