@@ -466,7 +466,9 @@ int sofie_b200_kv_append_enqueue(sofie_b200_ctx *ctx, const sofie_b200_kv_append
  * continued after lk - lq keys).  A query that sees no key gets zeros.  Keys and values that a query does not see have no
  * influence on it, whatever they hold (NaN and infinities included).
  * head_dim: a multiple of 8 up to 256; heads / kv_heads up to 64; token pitches multiples of 8 elements; tensors 16-byte aligned; up to
- * 2^27 query and key rows. */
+ * 2^27 query and key rows in all.  A sequence has up to 2^20 keys in bf16 and 2^24 in F32, behind which sums over so many keys would
+ * be off by more than the type's own steps; one with more is left out like one whose offsets are out of range (rows of y untouched,
+ * SOFIE_B200_ERR_DEVICE_INDEX).  SOFIE_B200_ERR_TOO_LARGE: bf16, and (query rows / queries of a tile + batch) * kv_heads above 2^27. */
 typedef struct sofie_b200_prompt_attention_desc {
   int32_t heads, kv_heads, head_dim;
   int32_t dtype;                 /* F32 or BF16 */

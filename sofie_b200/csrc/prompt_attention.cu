@@ -24,9 +24,19 @@ struct PromptParams {
   long long q_rows, k_rows;
   int batch, heads, kv_heads, dim, causal;
   int group, tokens;          // heads / kv_heads; queries of a tile
+  int most_keys;              // of a sequence
   float scale_log2e;
   int *status;
 };
+
+// Keys of a sequence at most.  bf16: the tensor cores cut what they add to a sum below its last bits, so that values of one sign under
+// equal weights lose n 2^-28 of it over n keys (measured 0.0039 at 2^20, half a step of the result's type; 0.023 at 2^22; half of
+// it at 2^27); and no wait may be as long as its limit of a second, though the warps of a tile of rows without a turn wait for all turns of
+// the block's other one: 1.71 us for 128 keys, 14 ms for 2^20 (and 1.79 s for 2^27).  fp32: sums in order, in which equal values count
+// exactly up to 2^24 (measured 1e-5 there, values of one sign).
+constexpr int MOST_KEYS_BF16 = 1 << 20, MOST_KEYS_F32 = 1 << 24;
+// Blocks of the bf16 kernel at most.  One without a tile takes 2.1 ns of the whole GPU's time, and the other warps wait for all of them: 0.28 s.
+constexpr long long MOST_BLOCKS = 1LL << 27;
 
 // One tile of queries: its sequence's rows, its first query and how many of them there are.
 struct PromptTile {
@@ -42,6 +52,7 @@ __device__ __forceinline__ int sequence_tiles(const PromptParams &p, int b, Prom
   bool bad = false;
   packed_range(p.cu_q, b, p.q_rows, &x0, &x1, &bad);
   packed_range(p.cu_k, b, p.k_rows, &y0, &y1, &bad);
+  bad |= x1 > x0 && y1 - y0 > p.most_keys;
   if (bad) report(p.status, DEV_BAD_INDEX);
   t.q0 = x0; t.k0 = y0; t.k_len = y1 - y0;
   q_len = bad ? 0 : x1 - x0;
@@ -1026,7 +1037,8 @@ static int launch_umma(sofie_b200_ctx *ctx, PromptParams p) {
   const int per = 128 / p.group;
   p.tokens = Cfg::TILES * per;
   const long long grid = (p.q_rows / p.tokens + p.batch) * p.kv_heads;   // every sequence may end inside a tile
-  if (grid > 0x7fffffffLL) return fail(SOFIE_B200_ERR_TOO_LARGE, "prompt_attention_enqueue: %lld queries of %d heads", p.q_rows, p.heads);
+  if (grid > MOST_BLOCKS)
+    return fail(SOFIE_B200_ERR_TOO_LARGE, "prompt_attention_enqueue: %lld queries of %d sequences and %d heads", p.q_rows, p.batch, p.heads);
   CUtensorMap tm_q, tm_k, tm_v;
   const void *k = p.k_rows ? p.k : p.q, *v = p.k_rows ? p.v : p.q;   // no keys: nothing is loaded, but a map has to describe something
   const long long k_rows = p.k_rows ? p.k_rows : 1;
@@ -1124,7 +1136,7 @@ int sofie_b200_prompt_attention_enqueue(sofie_b200_prompt_attention_plan *plan, 
                                         int64_t k_tokens) {
   if (!plan) return fail(SOFIE_B200_ERR_INVALID, "prompt_attention_enqueue: plan is NULL");
   const sofie_b200_prompt_attention_desc &d = plan->d;
-  if (batch < 0 || batch > 0x3fffffff || q_tokens < 0 || q_tokens > (1 << 27) || k_tokens < 0 || k_tokens > (1 << 27))   // a warp without rows waits for a tile's others: within the limit
+  if (batch < 0 || batch > 0x3fffffff || q_tokens < 0 || q_tokens > (1 << 27) || k_tokens < 0 || k_tokens > (1 << 27))
     return fail(SOFIE_B200_ERR_INVALID, "prompt_attention_enqueue: bad extent (batch %lld, %lld and %lld tokens)", (long long)batch,
                 (long long)q_tokens, (long long)k_tokens);
   if (batch == 0 || q_tokens == 0) return 0;
@@ -1140,6 +1152,7 @@ int sofie_b200_prompt_attention_enqueue(sofie_b200_prompt_attention_plan *plan, 
   p.q_rows = q_tokens; p.k_rows = k_tokens;
   p.batch = (int)batch; p.heads = d.heads; p.kv_heads = d.kv_heads; p.dim = d.head_dim; p.causal = d.causal != 0;
   p.group = d.heads / d.kv_heads;
+  p.most_keys = d.dtype == SOFIE_B200_BF16 ? MOST_KEYS_BF16 : MOST_KEYS_F32;
   p.scale_log2e = d.scale * 1.4426950408889634f;
   p.status = ctx->d_status;
   if (d.dtype == SOFIE_B200_BF16) {

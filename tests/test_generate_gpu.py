@@ -425,6 +425,51 @@ def test_prompt_far_rows(ctx):
         ref.close(y, *ref.prompt(q, k, v, [0, n], [0, n], True))
 
 
+def test_prompt_of_more_keys_than_a_sequence_has(ctx):
+    """2^27 keys in one bf16 sequence (19 GB): sums over so many would lose half of the result, and warps without a turn would wait for longer
+    than a second.  The sequence is left out and reported, the one behind it is not."""
+    from sofie_b200.ops import PromptAttentionPlan
+    n, dim = 1 << 27, 72
+    x = torch.ones((n, 1, dim), dtype=BF, device=DEV)   # keys and values
+    x[n // 2:] = 3.0
+    q, y = torch.zeros((2, 1, dim), dtype=BF, device=DEV), torch.full((2, 1, dim), 7.0, dtype=BF, device=DEV)
+    plan = PromptAttentionPlan(ctx, 1, 1, dim, BF)
+    for cu_k, left in (([0, n, n], (7.0, 0.0)), ([0, n - 4, n], (7.0, 3.0)), ([0, 4, (1 << 20) + 5], (1.0, 7.0))):
+        y.fill_(7.0)
+        plan.enqueue(q, x, x, y, ints([0, 1, 2]), ints(cu_k))
+        with pytest.raises(L.SofieB200Error) as e:
+            ctx.sync()
+        assert e.value.status == L.ERR_DEVICE_INDEX
+        assert (y[0] == left[0]).all() and (y[1] == left[1]).all()
+    plan.enqueue(q, x, x, y, ints([0, 0, 1]), ints([0, n - 4, n]))    # no queries: nothing to leave out
+    ctx.sync()
+    assert (y[0] == 3.0).all()
+
+
+@pytest.mark.parametrize("dtype,dim,most", [(BF, 64, 1 << 20), (BF, 128, 1 << 20), (BF, 256, 1 << 20), (F32, 8, 1 << 24)])
+def test_prompt_of_the_most_keys(ctx, dtype, dim, most):
+    """The longest sequence, equal weights, values of one sign: what sums over so many keys lose.  One key more is refused.
+    Bounds, relative to the result.  bf16: the tensor cores cut each product and each sum of 16 products by less than 2^-23 of the running
+    sum, which is half the result on average: n (17 / 16) 2^-24.  fp32: n / 2 sums in each of two teams of warps, each rounded by at
+    most 2^-24 of the result, either way as the random values fall: 8 sqrt(n / 2) 2^-24, eight standard deviations.  Then the
+    rounding of the result; the weights are 1."""
+    from sofie_b200.ops import PromptAttentionPlan
+    g = gen_of(3)
+    k = torch.zeros((most + 1, 1, dim), dtype=dtype, device=DEV)
+    v = (torch.rand((most + 1, 1, dim), generator=g, device=DEV) + 0.5).to(dtype)
+    q, y = torch.zeros((1, 1, dim), dtype=dtype, device=DEV), torch.full((1, 1, dim), 7.0, dtype=dtype, device=DEV)
+    plan = PromptAttentionPlan(ctx, 1, 1, dim, dtype)
+    plan.enqueue(q, k, v, y, ints([0, 1]), ints([0, most + 1]))
+    with pytest.raises(L.SofieB200Error) as e:
+        ctx.sync()
+    assert e.value.status == L.ERR_DEVICE_INDEX and (y == 7.0).all()
+    plan.enqueue(q, k, v, y, ints([0, 1]), ints([0, most]))
+    ctx.sync()
+    want = v[:most].double().mean(0, keepdim=True)
+    lost = most * 17 / 16 * 2.0 ** -24 if dtype is BF else 8 * math.sqrt(most / 2) * 2.0 ** -24
+    ref.close(y, want, (lost + ref.HALF[dtype]) * want)
+
+
 # ---- decode ---------------------------------------------------------------------------------------------------------
 DECODE = [
     # heads, kv_heads, dim, page_size, lengths, pages heads first
@@ -707,6 +752,16 @@ def test_prompt_extents_that_are_refused(ctx):
     for batch, n, m in ((-1, 8, 8), (1, -1, 8), (1, 8, -1), (1, (1 << 27) + 1, 8), (1, 8, (1 << 27) + 1), (1 << 30, 8, 8)):
         p = q.data_ptr()
         assert L.load().sofie_b200_prompt_attention_enqueue(plan._plan((0, 0, 0, 0)), p, p, p, p, cu.data_ptr(), cu.data_ptr(), batch, n, m) == L.ERR_INVALID
+    ctx.sync()
+
+
+def test_prompt_grids_that_are_refused(ctx):
+    """More blocks than are asked for one by one in the limit of a wait."""
+    from sofie_b200.ops import PromptAttentionPlan
+    q = torch.empty((8, 16, 8), dtype=BF, device=DEV)
+    cu, p = ints([0, 8]), q.data_ptr()
+    plan = PromptAttentionPlan(ctx, 16, 16, 8, BF)
+    assert L.load().sofie_b200_prompt_attention_enqueue(plan._plan((0, 0, 0, 0)), p, p, p, p, cu.data_ptr(), cu.data_ptr(), (1 << 23) + 1, 8, 8) == L.ERR_TOO_LARGE
     ctx.sync()
 
 
