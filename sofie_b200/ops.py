@@ -51,6 +51,13 @@ class Context:
             torch.cuda.current_stream(device).cuda_stream)
         L.check(self._lib.sofie_b200_ctx_create(C.byref(h), device, sp), "ctx_create")
         self._h = h
+        self._torch_stream = stream if stream is not None else torch.cuda.current_stream(device)
+
+    def scratch(self, size: int) -> torch.Tensor:
+        """Uninitialised device bytes that belong to the context's stream: of another stream's pool they could be a block that
+        was just freed there and is still written, and after their release one that this stream still uses."""
+        with torch.cuda.stream(self._torch_stream):
+            return torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
 
     def sync(self) -> None:
         L.check(self._lib.sofie_b200_ctx_sync(self._h), "ctx_sync")
@@ -132,7 +139,7 @@ class Context:
         h = C.c_void_p()
         L.check(self._lib.sofie_b200_sdpa_plan_create(self._h, C.byref(d), C.byref(h)), "sdpa_plan_create")
         try:
-            ws = torch.empty(max(256, self._lib.sofie_b200_sdpa_workspace_bytes(h)), dtype=torch.uint8, device=q.device)
+            ws = self.scratch(max(256, self._lib.sofie_b200_sdpa_workspace_bytes(h)))
             L.check(self._lib.sofie_b200_sdpa_enqueue(h, _ptr(q), _ptr(k), _ptr(v), _ptr(mask), _ptr(y), _ptr(ws)), "sdpa_enqueue")
             kernel = self._lib.sofie_b200_sdpa_plan_kernel(h).decode()
             self.sync()   # the workspace is released on return
@@ -393,9 +400,7 @@ class PagedAttentionPlan:
         h = self._plan((0, 0))
         size = int(self._lib.sofie_b200_paged_attention_workspace_bytes(h))
         if size:
-            self._workspace = torch.empty(size, dtype=torch.uint8, device=f"cuda:{ctx.device}")
-            if ctx.stream is not None:   # freed memory must not be handed out again while the context's stream still uses it
-                self._workspace.record_stream(ctx.stream)
+            self._workspace = ctx.scratch(size)
         self._workspace_ptr = _ptr(self._workspace)
 
     def _plan(self, pitches):

@@ -744,6 +744,34 @@ def test_two_graphs_replayed_side_by_side(b200_lib):
         r[1].close()
 
 
+def test_workspace_belongs_to_the_contexts_stream(b200_lib):
+    """Memory that was freed on the current stream, with a kernel there still to write it, is not the workspace of a plan on another stream."""
+    from sofie_b200.ops import Context, PagedAttentionPlan
+    for given in (True, False):   # the context's stream as an argument, and as the current one when the context was made
+        side = torch.cuda.Stream(device=DEV)
+        if given:
+            ctx = Context(0, stream=side)
+        else:
+            with torch.cuda.stream(side):
+                ctx = Context(0)
+        first = PagedAttentionPlan(ctx, 8, 2, 128, BF)
+        size = first._workspace.numel()
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        old = torch.empty(size, dtype=torch.uint8, device=DEV)
+        begin, end = old.data_ptr(), old.data_ptr() + size
+        torch.cuda._sleep(50_000_000)
+        old.fill_(1)
+        del old
+        plan = PagedAttentionPlan(ctx, 8, 2, 128, BF)
+        at = plan._workspace.data_ptr()
+        assert at + size <= begin or at >= end
+        torch.cuda.synchronize()
+        for p in (first, plan):
+            p.close()
+        ctx.close()
+
+
 def test_prompt_extents_that_are_refused(ctx):
     from sofie_b200.ops import PromptAttentionPlan
     q = torch.empty((8, 1, 8), dtype=BF, device=DEV)
