@@ -229,7 +229,8 @@ int sofie_b200_ctx_destroy(sofie_b200_ctx *ctx);
  * RModel_ALPAKA.cxx:857-909) and returns SOFIE_B200_ERR_DEVICE_WAIT if a kernel reported a
  * bounded wait that ran out since the last call, or SOFIE_B200_ERR_DEVICE_INDEX if one met a page, length or
  * offset in device memory that is out of range (the generation operators check what they read from
- * block tables and length arrays, leave out the access, and carry on). */
+ * block tables and length arrays, leave out the access, and carry on).  Where both happened it is SOFIE_B200_ERR_DEVICE_WAIT:
+ * results are unfinished. */
 int sofie_b200_ctx_sync(sofie_b200_ctx *ctx);
 
 /* Number of kernels this ctx has launched so far (for launch accounting in benchmarks). */

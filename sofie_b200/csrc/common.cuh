@@ -34,6 +34,12 @@ enum DeviceStatus : int {
   DEV_BAD_INDEX = 5,        // a page, length or offset read from device memory was out of range; the access was left out
 };
 
+// Writes a code to the context's status word.  The first one stays, but a wait that ran out, whose results are unfinished, takes the place of a bad
+// index, which was left out and hurt nothing else.
+__device__ __forceinline__ void report(int *status, int code) {
+  if (atomicCAS(status, DEV_OK, code) == DEV_BAD_INDEX && code != DEV_BAD_INDEX) atomicCAS(status, DEV_BAD_INDEX, code);
+}
+
 inline int dtype_size(int dt) {
   switch (dt) {
     case SOFIE_B200_F32: return 4;

@@ -5,9 +5,6 @@
 
 namespace sb200 {
 
-// Writes a code to the context's status word unless one is there already.
-__device__ __forceinline__ void report(int *status, int code) { atomicCAS(status, 0, code); }
-
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void from_f32(float *p, float x) { *p = x; }

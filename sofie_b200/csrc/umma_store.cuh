@@ -8,7 +8,7 @@ namespace sb200 {
 
 __device__ __forceinline__ void raise_abort(volatile int *abort_flag, int *status, int code) {
   *abort_flag = 1;
-  atomicCAS(status, 0, code);
+  report(status, code);
 }
 
 __device__ __forceinline__ void st_v4(void *p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {

@@ -744,6 +744,28 @@ def test_two_graphs_replayed_side_by_side(b200_lib):
         r[1].close()
 
 
+@pytest.mark.parametrize("wait_first", [True, False])
+def test_a_wait_that_ran_out_is_reported_before_a_bad_index(ctx, wait_first):
+    """Both in one step, in either order: the caller hears of the results that are unfinished."""
+    from sofie_b200.ops import PagedKV
+    ck, cv, k = (torch.zeros(s, dtype=BF, device=DEV) for s in ((2, 4, 1, 8), (2, 4, 1, 8), (1, 1, 8)))
+    kv = PagedKV(ck, cv, ints([[9]]), ints([1]))
+
+    def wait():
+        assert L.load().sofie_b200_selftest_wait_timeout(ctx._h, 1000) == 0   # a bounded wait on a barrier that nothing signals
+
+    for call in (wait, lambda: ctx.kv_append(k, k, kv))[::1 if wait_first else -1]:
+        call()
+    with pytest.raises(L.SofieB200Error) as e:
+        ctx.sync()
+    assert e.value.status == L.ERR_DEVICE_WAIT
+    ctx.sync()
+    ctx.kv_append(k, k, kv)
+    with pytest.raises(L.SofieB200Error) as e:
+        ctx.sync()
+    assert e.value.status == L.ERR_DEVICE_INDEX
+
+
 def test_workspace_belongs_to_the_contexts_stream(b200_lib):
     """Memory that was freed on the current stream, with a kernel there still to write it, is not the workspace of a plan on another stream."""
     from sofie_b200.ops import Context, PagedAttentionPlan
