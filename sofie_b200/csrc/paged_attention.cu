@@ -202,7 +202,8 @@ struct Bf16Cfg {
 
 // bf16.  Scores and weighted values on mma.m16n8k16 with the 16 rows = query heads of the group (rows past the group cost nothing that HBM
 // would not wait for).  The weights of the second product are split into two bf16 terms, high + low (error 2^-16 instead of 2^-8):
-// the tensor cores have the time.
+// the tensor cores have the time.  The high term is cut, not rounded, and the low one kept above zero (by 2^-20 of the weight), so that
+// both have the weight's sign and an infinite value comes out infinite: 0 * inf and inf - inf are NaN.  As fast as rounding (230, 61.5 us).
 // Bound by HBM; at head size 128 the rings of two blocks are 192 KB an SM, two thirds of it on the way.  160 sequences, 1.22 GB of cache:
 // 209 to 230 us, 5.3 to 5.8 TB/s (DRAM 75 % busy, issue slots 42 %, tensor pipe 28 %); one of 65,543 tokens, 268 MB: 61 us with the launch of
 // both kernels, 4.4 TB/s.  A fixed split of every sequence into equal parts, one block each: 66 and 236 us.
@@ -299,9 +300,9 @@ __global__ void __launch_bounds__(128) paged_mma_kernel(const __grid_constant__ 
           const float e0 = ex2(s[t][2 * half] - mm), e1 = ex2(s[t][2 * half + 1] - mm);
           if (half) l1 += e0 + e1;
           else l0 += e0 + e1;
-          const __nv_bfloat162 h = __floats2bfloat162_rn(e0, e1);
-          const __nv_bfloat162 r = __floats2bfloat162_rn(e0 - __low2float(h), e1 - __high2float(h));
-          hi[t * 2 + half] = *reinterpret_cast<const uint32_t *>(&h);
+          const float h0 = __uint_as_float(__float_as_uint(e0) & 0xffff0000u), h1 = __uint_as_float(__float_as_uint(e1) & 0xffff0000u);
+          const __nv_bfloat162 r = __floats2bfloat162_rn(fmaxf(e0 - h0, e0 * 0x1p-20f), fmaxf(e1 - h1, e1 * 0x1p-20f));
+          hi[t * 2 + half] = __byte_perm(__float_as_uint(e0), __float_as_uint(e1), 0x7632);
           lo[t * 2 + half] = *reinterpret_cast<const uint32_t *>(&r);
         }
       // ---- weighted values: 16 rows x DP ----

@@ -533,6 +533,35 @@ def test_decode(ctx, case, dtype):
     plan.close()
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("heads,kvh,dim,lens", [(4, 1, 64, [1, 17, 300]), (8, 2, 128, [40, 3000]), (20, 1, 80, [500, 9]), (3, 1, 256, [33, 2000]), (1, 1, 8, [40000, 2])])
+def test_decode_values_that_are_not_finite(ctx, dtype, heads, kvh, dim, lens):
+    """Infinite and NaN values that a sequence sees come out in their dimension; everything else is what it is without them."""
+    from sofie_b200.ops import PagedAttentionPlan, PagedKV
+    q, ck, cv, table = decode_case(heads, kvh, dim, 16, lens, False, dtype, 91)
+    clean = cv.clone()
+    expect = []
+    for b, n in enumerate(lens):
+        for at, d, value in ((0, 0, math.inf), (n // 2, 3, -math.inf), (n - 1, 5, math.inf), (n // 3, 6, math.nan)):
+            where = int(table[b, at // 16]), at % 16, slice(None), d
+            cv[where], clean[where] = value, 0.0
+            expect.append((b, d, value))
+        if n > 1:
+            for at, value in ((0, math.inf), (n - 1, -math.inf)):
+                where = int(table[b, at // 16]), at % 16, slice(None), 7
+                cv[where], clean[where] = value, 0.0
+            expect.append((b, 7, math.nan))
+    want, tol = ref.decode(q, ck, clean, table, lens)
+    y = torch.empty_like(q)
+    PagedAttentionPlan(ctx, heads, kvh, dim, dtype).enqueue(q, PagedKV(ck, cv, table, ints(lens)), y)
+    ctx.sync()
+    for b, d, value in expect:
+        got = y[b, :, d].double()
+        assert (got.isnan() if math.isnan(value) else got == value).all(), (b, d, value)
+        want[b, :, d], y[b, :, d] = 0.0, 0.0
+    ref.close(y, want, tol)
+
+
 def test_decode_leaves_out_bad_pages(ctx):
     from sofie_b200.ops import PagedAttentionPlan, PagedKV
     for dtype in (BF, F32):
