@@ -140,7 +140,12 @@ class ConvNetB200:
         self.keep.append(k)
 
     def __call__(self, x):
-        """x: [batch, 3, img, img] on the device; returns the logits buffer (owned here, overwritten by the next call)."""
+        """x: [batch, 3, img, img] on the device; returns the logits buffer (owned here, overwritten by the next call).  Work is only
+        enqueued, on the context's stream and in order with the current one."""
+        with self.ctx.in_order():
+            return self._enqueue(x)
+
+    def _enqueue(self, x):
         from sofie_b200 import lib as L
         cur = x
         for h, ep, y in zip(self.plans, self.eps, self.acts):

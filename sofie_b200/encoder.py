@@ -105,7 +105,11 @@ class EncoderB200:
 
     def __call__(self, x):
         """x: [batch*seq, d_model] bf16 on the device; returns the output activations (a buffer owned by this object,
-        overwritten by the next call).  Work is only enqueued; the caller synchronises."""
+        overwritten by the next call).  Work is only enqueued, on the context's stream and in order with the current one."""
+        with self.ctx.in_order():
+            return self._enqueue(x)
+
+    def _enqueue(self, x):
         ctx, heads, b, s, dh = self.ctx, self.heads, self.batch, self.seq, self.dh
         m = b * s
         cur = x

@@ -5,6 +5,7 @@ libsofie_b200.so.  Tensors must live on the context's CUDA device.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import numpy as np
@@ -52,6 +53,18 @@ class Context:
         L.check(self._lib.sofie_b200_ctx_create(C.byref(h), device, sp), "ctx_create")
         self._h = h
         self._torch_stream = stream if stream is not None else torch.cuda.current_stream(device)
+
+    @contextlib.contextmanager
+    def in_order(self):
+        """What is enqueued inside runs behind the current stream's work so far and before what comes there later, as torch's own
+        operators do.  Nothing to do where the context's stream is the current one (also under capture)."""
+        current = torch.cuda.current_stream(self.device)
+        apart = current != self._torch_stream and not torch.cuda.is_current_stream_capturing()
+        if apart:
+            self._torch_stream.wait_stream(current)
+        yield
+        if apart:
+            current.wait_stream(self._torch_stream)
 
     def scratch(self, size: int) -> torch.Tensor:
         """Uninitialised device bytes that belong to the context's stream: of another stream's pool they could be a block that

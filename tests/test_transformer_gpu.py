@@ -112,6 +112,41 @@ def test_encoder_step_replays_from_a_cuda_graph(b200_lib):
     ctx.close()
 
 
+def test_encoder_runs_in_order_with_the_current_stream(b200_lib):
+    """A context on a stream of its own: the current stream's work on the input comes before a call, and what it does with the result
+    (and with the input) afterwards comes behind, also while the context's stream is busy."""
+    from sofie_b200 import encoder as be
+    from sofie_b200.ops import Context
+    rng = np.random.default_rng(21)
+    weights = be.make_weights(6, LAYERS, D_MODEL, FFN)
+    bits = [be.f32_to_bf16_bits(rng.standard_normal((B * S, D_MODEL)).astype(np.float32)) for _ in range(2)]
+    xs = [torch.from_numpy(b.view(np.int16)).to(DEV).view(torch.bfloat16) for b in bits]
+    side = torch.cuda.Stream(device=DEV)
+    ctx = Context(0, stream=side)
+    enc = be.EncoderB200(ctx, weights, B, S, D_MODEL, HEADS, FFN, DEV, fused_attention=True)
+    torch.cuda.synchronize()
+    want = []
+    for x in xs:
+        y = enc(x)
+        torch.cuda.synchronize()
+        want.append(y.clone())
+    torch.cuda.synchronize()
+    cur = torch.empty_like(xs[0])
+    got = []
+    for x in xs:
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+        torch.cuda._sleep(20_000_000)
+        cur.copy_(x)
+        got.append(enc(cur).clone())
+        cur.zero_()
+    ctx.sync()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    enc.close()
+    ctx.close()
+
+
 @pytest.mark.parametrize("shape,perm", [((2, 128, 24, 64), (2, 0, 1, 3)), ((8, 2, 128, 64), (1, 2, 0, 3)), ((5, 7, 9), (2, 0, 1)),
                                         ((33, 65), (1, 0)), ((3, 4, 5, 6), (3, 2, 1, 0))])
 def test_transpose(b200_lib, shape, perm):
