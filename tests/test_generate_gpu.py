@@ -409,6 +409,26 @@ def test_prompt_bad_offsets_are_left_out(ctx):
                 assert err.status == L.ERR_DEVICE_INDEX
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("cu,good", [([0, 30, 20], [(0, 30)]), ([-5, 20, 50], [(20, 50)]), ([0, 2000000000, 50], []), ([0, 20, 51], [(0, 20)]),
+                                     ([0, 20, -1], [(0, 20)]), ([50, 0, 50], [(0, 50)])])
+def test_prompt_refused_offsets_leave_the_others(ctx, dtype, cu, good):
+    """Every list says so at the next sync; sequences whose offsets are in order come out, the rows of no such sequence stay."""
+    from sofie_b200.ops import PromptAttentionPlan
+    q, k, v, _, _ = prompt_case(4, 2, 64, [20, 30], None, dtype, 6, spare=0)
+    y = torch.full_like(q, 3.0)
+    PromptAttentionPlan(ctx, 4, 2, 64, dtype).enqueue(q, k, v, y, ints(cu))
+    with pytest.raises(L.SofieB200Error) as e:
+        ctx.sync()
+    assert e.value.status == L.ERR_DEVICE_INDEX
+    stays = torch.ones(50, dtype=torch.bool, device=DEV)
+    for s, t in good:
+        want, tol = ref.prompt(q[s:t], k[s:t], v[s:t], [0, t - s], [0, t - s], True)
+        ref.close(y[s:t], want, tol)
+        stays[s:t] = False
+    assert (y[stays] == 3.0).all()
+
+
 def test_prompt_far_rows(ctx):
     """Element offsets past 2^31: a token pitch of 2^23 elements."""
     from sofie_b200.ops import PromptAttentionPlan
