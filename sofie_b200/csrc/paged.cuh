@@ -93,7 +93,8 @@ SB_HD int split_last(long long slots, int workers, long long end) {
   return lo;
 }
 
-// Workers that get work: none fewer than `least` slots, unless there are fewer in all.
+// Workers that get work: as many as shares of `least` slots make, the last one begun counting as one.  So a share may be smaller (4
+// slots by 3: two of 2), but holds at least half of `least`, unless there are fewer slots in all.
 SB_HD int split_workers(long long slots, int workers, int least) {
   const long long most = quotient(slots + least - 1, least);
   return most < 1 ? 1 : most < workers ? (int)most : workers;

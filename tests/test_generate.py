@@ -344,3 +344,36 @@ int main() {
 
 def test_dealing_of_the_cache_to_warps(tmp_path):
     build_and_run(tmp_path, SPLIT)
+
+
+WORKERS = r'''
+#include "paged.cuh"
+#include <algorithm>
+#include <cstdio>
+using namespace sb200;
+#define NEED(c) do { if (!(c)) { printf("failed: %s (line %d)\n", #c, __LINE__); return 1; } } while (0)
+int main() {
+  for (int least = 1; least <= 9; ++least)
+    for (int all : {1, 2, 7, 100, 1184})
+      for (long long slots : {1LL, 2LL, 3LL, 4LL, 5LL, 7LL, 8LL, 10LL, 11LL, 16LL, 19LL, 100LL, 101LL, 1184LL, 3551LL, 3553LL, 1LL << 40}) {
+        const int n = split_workers(slots, all, least);
+        NEED(n >= 1 && n <= all && (n == all || (long long)n * least >= slots) && (n - 1LL) * least < slots);
+        long long smallest = slots, sum = 0;
+        for (int c = 0; c < n; ++c) {
+          const long long share = split_at(slots, n, c + 1) - split_at(slots, n, c);
+          smallest = std::min(smallest, share);
+          sum += share;
+        }
+        NEED(sum == slots);
+        NEED(2 * smallest >= std::min<long long>(least, slots));
+      }
+  NEED(split_workers(4, 100, 3) == 2 && split_at(4, 2, 1) == 2);
+  NEED(split_workers(0, 100, 3) == 1);
+  puts("ok");
+  return 0;
+}
+'''
+
+
+def test_shares_hold_half_of_the_least_that_is_worth_a_worker(tmp_path):
+    build_and_run(tmp_path, WORKERS)
