@@ -422,7 +422,10 @@ int sofie_b200_sdpa_enqueue(sofie_b200_sdpa_plan *plan, const void *q, const voi
  *   seq_lens     int32 [batch]: tokens of sequence b in the cache, the ones being appended included
  *   block_table  int32 [batch, table_width]: token p of sequence b lives in page block_table[b][p / page_size], slot p % page_size
  * Grouped heads: query head h reads key head h / (heads / kv_heads).  Types F32 and BF16, one for all tensors of a call; scores,
- * row maxima, row sums and results are held in fp32 and rounded once.
+ * row maxima, row sums and results are held in fp32 and rounded once.  In BF16 the weights are rounded for their product with the
+ * values as well (the row sums add them unrounded): to bf16, half a step of the result's type, in prompt attention; to two bf16 terms,
+ * 2^-16, in attention over the cache.
+ * Token pitches and table_pitch: 0 = dense; rows do not lie over one another.
  * Indices in device memory cannot be refused by the host.  The kernels check them: a token whose page, position or row is out of
  * range is left out (not written, not attended to), every other one is processed, and the next sofie_b200_ctx_sync returns
  * SOFIE_B200_ERR_DEVICE_INDEX.
@@ -464,8 +467,9 @@ int sofie_b200_kv_append_enqueue(sofie_b200_ctx *ctx, const sofie_b200_kv_append
 
 /* Attention over packed prompts: y[i,h] = sum_j softmax_j(scale q[i,h] . k[j, h / g]) v[j, h / g] over the keys j of query i's own
  * sequence -- all lk of them, or with causal = 1 those with j <= i + lk - lq (the last query sees the last key; lk > lq: a prompt
- * continued after lk - lq keys).  A query that sees no key gets zeros.  Keys and values that a query does not see have no
- * influence on it, whatever they hold (NaN and infinities included).
+ * continued after lk - lq keys).  Keys and values are packed rows: earlier ones that lie in the paged cache are gathered into a
+ * copy by the caller first, the whole of each sequence's keys in order.  A query that sees no key gets zeros.  Keys and values that
+ * a query does not see have no influence on it, whatever they hold (NaN and infinities included).
  * head_dim: a multiple of 8 up to 256; heads / kv_heads up to 64; token pitches multiples of 8 elements; tensors 16-byte aligned; up to
  * 2^27 query and key rows in all.  A sequence has up to 2^20 keys in bf16 and 2^24 in F32, behind which sums over so many keys would
  * be off by more than the type's own steps; one with more is left out like one whose offsets are out of range (rows of y untouched,
@@ -490,7 +494,8 @@ int sofie_b200_prompt_attention_enqueue(sofie_b200_prompt_attention_plan *plan, 
 
 /* Attention of one new token per sequence over the paged cache: y[b,h] = the sum above over the seq_lens[b] tokens of sequence b in
  * the cache.  seq_lens[b] = 0 (a padding row) gives zeros.  The cache's length is split over the GPU whatever the batch is, and the
- * parts are joined in a fixed order (the same inputs give the same bits).
+ * parts are joined in a fixed order (the same inputs give the same bits).  Keys and values are read once for every 16 query heads that
+ * share them.
  * head_dim: a multiple of 8 up to 256; heads / kv_heads up to 64; strides and pitches multiples of 8 elements; tensors 16-byte aligned. */
 typedef struct sofie_b200_paged_attention_desc {
   int32_t heads, kv_heads, head_dim;

@@ -118,8 +118,9 @@ struct alignas(sizeof(T) * V) Piece {
 // with the V of the second half that turn with them (or V / 2 neighbouring pairs), so q_out may be q; or V elements that are only
 // copied.  A thread has the same unit of several heads, so its angles are loaded once.  Bound by HBM where tokens are many: every element
 // is read once and written once, 16 bytes at a time where the layout allows it; what keeps it from the copy rate is that a thread
-// waits for its loads, two heads at a time (more take registers, and with them warps: 4 heads 79 us, 2 heads 63 us at 10,832 tokens of
-// 32 + 2 x 8 heads of 128 in bf16 = 4.3 TB/s).  The first heads are on their way before the token's place is known, which takes two or
+// waits for its loads, two heads at a time (more take registers, and with them warps: 4 heads 79 us, 2 heads 62 us at 10,832 tokens of
+// 32 + 2 x 8 heads of 128 in bf16 = 4.4 TB/s).  Even so that form, <bf16, 8, 64>, spills at its 64 registers: 150 bytes of stores and 200 of
+// loads a thread, as the pieces of values and the angles are held across the look-up of the token's place.  The first heads are on their way before the token's place is known, which takes two or
 // three rounds of dependent loads.
 template <class T, int V, int GROUP>
 __global__ void __launch_bounds__(256, GROUP < 256 ? 4 : 1) kv_append_kernel(const __grid_constant__ AppendParams p) {

@@ -1,7 +1,7 @@
 // Attention of one new token per sequence over a paged key-value cache:
 //     y[b, h] = sum_j softmax_j(scale q[b, h] . k[j, h / g]) v[j, h / g],   j < seq_lens[b],   g = heads / kv_heads.
-// Each key and value is read once for the g query heads that share it, so the kernel is bound by HBM: 2 D elements per token and
-// key head for 4 g D operations.
+// Each key and value is read once for the query heads that share it, 16 of them at a time (a larger group reads it once for every 16), so
+// the kernel is bound by HBM: 2 D elements per token and key head for 4 g D operations.
 //
 // Split.  One sequence may be the whole batch and 65,000 tokens long, or a batch may hold hundreds of very different lengths.
 // The tokens of all sequences and key heads are one row of units of 16 keys, cut into equal shares, one for every resident warp

@@ -471,8 +471,9 @@ struct UmmaSize : UmmaCfg<DP> {
   static constexpr int Q = C::TILES * PANELS * 16384;
   static constexpr int TILE = C::KEYS * DP * 2;             // keys or values
   static constexpr int PANEL = C::KEYS * 128;
-  // Warps of rows; then TMA, MMA.  Where a thread holds a row of 128 scores, 168 registers (12 warps' share) make it spill: the block
-  // is launched with a whole third group of warps, which hands registers over, 384 x 168 = 256 x 200 + 128 x 104.
+  // Warps of rows; then TMA, MMA.  Where a thread holds a row of 128 scores it needs more than 168 registers (12 warps' share): the block
+  // is launched with a whole third group of warps, which hands registers over, 384 x 168 = 256 x 200 + 128 x 104.  The compiler still
+  // allots 168 and spills a little, 104 bytes of stores and 156 of loads a thread.
   static constexpr bool MOVE = C::TILES == 2;
   static constexpr int THREADS = C::TILES * 128 + (MOVE ? 128 : 64);
   static constexpr int CONTROL = 512 + 64 + 64 + 4 * (RUNS + 1);   // barriers, mail, answers, table of tiles
@@ -529,7 +530,7 @@ __device__ __noinline__ void add_nonfinite(const PromptParams &p, long long q_ro
 // The reference maximum of a row moves only when a tile's maximum is 2^16 above it (fp32 and bf16 keep their relative precision up
 // there, and numerator and denominator use the same); then O is rescaled in tensor memory, which is rare.
 // Only tiles that the sequence's end or the diagonal cross pay for masks.  Every wait has a limit.
-// Measured: a causal prompt of 8192 tokens, 32 heads over 8 of 128, 494 to 505 us in bursts = 1.09 to 1.11 PFLOP/s (572 us under the power limit),
+// Measured: a causal prompt of 8192 tokens, 32 heads over 8 of 128, 558 to 563 us back to back = 0.98 PFLOP/s (494 to 505 us in short bursts),
 // tensor pipe 51 % (60 % with its operand traffic), exponentials 51 %: the two rows' chains of maximum, exponential and hand-over
 // fill the gaps of one another only in part.  24 packed prompts of 5 to 2500 tokens 133 us; 512 sequences of 24 to 128, head size 64, full,
 // 131 MB: 60 us (a tile is two turns, so beginning and ending it is what counts).
@@ -695,7 +696,10 @@ prompt_umma_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
               tc_fence_after();
             }
           }
-          auto weigh = [&](int at, float2 off2, float2 &sum) {   // 32 scores -> 16 columns of P
+          // 32 scores -> 16 columns of P.  The weights are rounded to bf16: the second product takes both operands in the values' type.  That is
+          // half a step of the result's type; against 64 bits results were off by 0.0018 to 0.0021 where fp32 weights give 0.0016 (prompts of
+          // 40 to 8192 tokens).  Two terms, as over the cache, would double that product and need columns that head size 128 does not have.
+          auto weigh = [&](int at, float2 off2, float2 &sum) {
             uint32_t w[16];
             float2 other = make_float2(0.f, 0.f);
 #pragma unroll
